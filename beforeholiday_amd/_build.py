@@ -71,6 +71,9 @@ def write_ninja() -> str:
     hip_flags = [
         opt, f"--offload-arch={arch}", "-std=c++17", "-fPIC", "-ffp-contract=fast",
         "-D__HIP_PLATFORM_AMD__=1", "-munsafe-fp-atomics", "-Wno-unused-result",
+        # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): some of its forms have given wrong results on
+        # MI355X now and then. The host pass warns that it does not know the feature: harmless.
+        "-Xclang -target-feature -Xclang -packed-fp32-ops",
         f"-I{os.path.join(CSRC, 'include')}",
     ]
     cxx_flags = [
