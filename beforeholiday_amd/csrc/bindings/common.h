@@ -68,5 +68,6 @@ void register_misc(pybind11::module_& m);
 void register_conv(pybind11::module_& m);
 void register_conv_bn(pybind11::module_& m);
 void register_bn_fold(pybind11::module_& m);
+void register_decoder_ops(pybind11::module_& m);
 
 }  // namespace bhb

@@ -18,4 +18,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bhb::register_conv(m);
   bhb::register_conv_bn(m);
   bhb::register_bn_fold(m);
+  bhb::register_decoder_ops(m);
 }

@@ -1,0 +1,779 @@
+// Grouped-query attention, forward and recomputing backward (gfx950, MFMA 32x32x16).
+//
+//   S = scale Q K^T,  P = softmax of S over the keys a query sees,  O = (P * keep / (1 - p)) V
+//   dV = Pd^T dO,  dP = (dO V^T) * keep / (1 - p),  delta = rowsum(dO * O),  dS = P (dP - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q
+//
+// The forward keeps one number per query, L = log2 sum 2^(scale log2(e) s); the backward rebuilds
+// P = 2^(scale log2(e) s - L). Scores, sums, L, delta and every accumulator are fp32; P and dS are rounded to
+// the tensors' 16-bit type where they enter a matrix product (their rounding errors are independent and
+// average out over the keys, like the rounding of the inputs).
+#include "bh/api.h"
+#include "bh/grouped_attn_api.h"
+#include "bh/mfma32.h"
+
+#include <algorithm>
+#include <type_traits>
+#include <stdexcept>
+#include <string>
+
+namespace bh {
+namespace {
+
+using namespace m32;
+
+constexpr int kThreads = 256;  // 4 waves
+constexpr int kTileQ = 128;    // rows of a workgroup: 32 per wave
+constexpr int kBlk = 64;       // rows of the streamed operand per step
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- LDS images ------------------------------------------------------------------------------------------
+// Row-major, 2 D bytes a row, 16-byte chunks XOR-swizzled by the row so that both reads are conflict free:
+// 16 consecutive rows of one chunk (ds_read_b128) land in 16 different slots, and the 4 consecutive rows x
+// 64 bytes of a transposed read (ds_read_b64_tr_b16) in 4 different quarters of the 256-byte bank line.
+template <int D> BH_HD constexpr int swz(int row) {
+  return D == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
+}
+template <int D> struct Frag {
+  static constexpr int RB = 2 * D;
+  int r0, lo, hi;  // this lane's byte offsets; the swizzle only mixes chunk bits, so a step is one XOR
+  BH_DEVICE explicit Frag(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    r0 = r * RB + ((h ^ swz<D>(r)) << 4);
+    const int g = (lane >> 4) & 1, q = (lane & 15) >> 2, p = lane & 3;
+    const int row = 4 * h + q, ch = 2 * g + (p >> 1), b = (p & 1) << 3;
+    lo = row * RB + ((ch ^ swz<D>(row)) << 4) + b;
+    hi = (row + 8) * RB + ((ch ^ swz<D>(row + 8)) << 4) + b;
+  }
+  // rows `row0 ..+31`, columns 16 s ..+15 as a row operand (row0 a multiple of 16)
+  BH_DEVICE i4v row(const char* img, int row0, int s) const {
+    return *reinterpret_cast<const i4v*>(img + row0 * RB + (r0 ^ (s << 5)));
+  }
+  // columns 32 dn ..+31 as rows, k = image rows k0 ..+15 in the register order of an accumulator tile
+  BH_DEVICE i4v tr(const char* img, int k0, int dn) const {
+    const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(img + k0 * RB + (lo ^ (dn << 6))));
+    const s4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(img + k0 * RB + (hi ^ (dn << 6))));
+    const i2v x = __builtin_bit_cast(i2v, a), y = __builtin_bit_cast(i2v, b);
+    return i4v{x[0], x[1], y[0], y[1]};
+  }
+};
+
+// LDS-DMA of ROWS rows of one operand by NW waves (wave index w of them): rows past the tensor's last and
+// columns past the head size land as zeros. Offsets stay below 2^31 for row strides below 2^24 elements
+// (checked on the host); the 64-bit part of the address is in the resource's base.
+template <int D, int ROWS, int NW> struct Stage {
+  static constexpr int RB = 2 * D, CH = RB / 16, NP = ROWS * RB / 1024 / NW;
+  int voff[NP];
+  BH_DEVICE Stage(int64_t st, int hn, int w, int lane) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int row = (w * NP + i) * (64 / CH) + lane / CH, ch = (lane % CH) ^ swz<D>(row);
+      voff[i] = 8 * ch < hn ? row * (int)st * 2 + ch * 16 : kOutOfRange;
+    }
+  }
+  template <typename T>
+  BH_DEVICE void issue(const T* base, int64_t st, int hn, int valid, const char* img, int w) const {
+    const int n = min(valid, ROWS);
+    const i4v rs = make_rsrc(base, n > 0 ? (uint32_t)(((n - 1) * (int)st + hn) * 2) : 0u);
+    const unsigned l = __builtin_amdgcn_readfirstlane(lds_addr(img) + w * (NP * 1024));
+#pragma unroll
+    for (int i = 0; i < NP; ++i) dma16(rs, voff[i], l + i * 1024);
+  }
+};
+
+// 8 columns of one row straight from memory as a matrix operand; zeros past the head size or the last row
+template <typename T> BH_DEVICE i4v load_frag(const T* base, int64_t st, int row, int rows, int col, int hn) {
+  if (row < rows && col < hn) return *reinterpret_cast<const i4v*>(base + (int64_t)row * st + col);
+  return i4v{0, 0, 0, 0};
+}
+
+template <typename T> BH_DEVICE T* at(const GaView& v, int b, int h) {
+  return reinterpret_cast<T*>(v.p) + (int64_t)b * v.sb + (int64_t)h * v.sh;
+}
+BH_DEVICE uint64_t eff_seed(const GaArgs& a) {
+  return a.seed_dev ? a.seed ^ ((uint64_t)*a.seed_dev * 0x9E3779B97F4A7C15ull) : a.seed;
+}
+BH_DEVICE int seq_keys(const GaArgs& a, int b) {
+  return a.lens ? __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.sk)) : a.sk;
+}
+
+// Problem of a workgroup on a 1-D grid of nx tiles x (b * ng) key heads x per heads. Workgroups go round-robin
+// to the 8 XCDs, each with an L2 of its own, so the tiles and query heads that read one key head's K / V stay
+// on one XCD where the count of key heads allows. tile_major: all problems' tile 0 first (causal: heaviest
+// tiles first, the light ones fill the gaps at the end), else a key head's tiles run together.
+struct Problem {
+  int tile, unit, j;
+};
+BH_DEVICE Problem problem(int nx, int units, int per, bool tile_major) {
+  const int id = blockIdx.x;
+  const int nxcd = (units & 7) == 0 ? 8 : 1;
+  const int xcd = id % nxcd, slot = id / nxcd, u = units / nxcd;
+  Problem p;
+  if (tile_major) {
+    p.tile = slot / (u * per);
+    const int rem = slot - p.tile * (u * per);
+    p.unit = rem / per * nxcd + xcd;
+    p.j = rem % per;
+  } else {
+    p.unit = slot / (nx * per) * nxcd + xcd;
+    const int rem = slot % (nx * per);
+    p.tile = rem / per;
+    p.j = rem % per;
+  }
+  return p;
+}
+
+// masks the scores of one 32-key (32-query) tile whose register i stands for offset acc_row(i): keeps
+// lo <= offset <= hi
+BH_DEVICE void mask_hi(f16v& s, int hi) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (acc_row(i) > hi) s[i] = -INFINITY;
+}
+BH_DEVICE void mask_lo(f16v& s, int lo) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (acc_row(i) < lo) s[i] = -INFINITY;
+}
+BH_DEVICE float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+BH_DEVICE float tile_max(const f16v& s) {
+  const float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]), c = max3(s[6], s[7], s[8]);
+  const float d = max3(s[9], s[10], s[11]), e = max3(s[12], s[13], s[14]);
+  return max3(max3(a, b, c), max3(d, e, s[15]), s[15]);
+}
+
+// ---- forward ---------------------------------------------------------------------------------------------
+// Workgroup = 4 waves x 32 queries of one head, the query on the lane: S^T = K Q^T puts a query's scores of a
+// 64-key block into one lane pair's registers, so the softmax needs one half-wave exchange and P^T feeds
+// O^T = V^T P^T from the accumulators. The running maximum is only raised when some query's block maximum
+// passes it by more than 2^8 (P <= 256 rounds as well as P <= 1; a wave-uniform vote).
+// K / V blocks arrive by LDS-DMA one block ahead: one barrier a block.
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32_t thresh, float kscale) {
+  constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
+  __shared__ __attribute__((aligned(16))) char smem[4 * IMG];  // {K, V} x 2 buffers
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int r = a.np / a.ng;
+  Problem pr = problem(nx, a.b * a.ng, r, a.causal);
+  if (a.causal) pr.tile = nx - 1 - pr.tile;
+  const int b = pr.unit / a.ng, g = pr.unit % a.ng, head = g * r + pr.j, bh = b * a.np + head;
+  const int nk = seq_keys(a, b), off = a.sk - a.sq;
+  const int q0 = pr.tile * kTileQ, q0w = q0 + wave * 32, myq = q0w + r32, pos = myq + off;
+  const int qlw = min(q0w + 31, a.sq - 1);  // the wave's last query
+
+  const T* K = at<const T>(a.k, b, g);
+  const T* V = at<const T>(a.v, b, g);
+  const T* Q = at<const T>(a.q, b, head);
+  i4v qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = load_frag<T>(Q, a.q.st, myq, a.sq, 16 * s + 8 * h, a.hn);
+
+  const float c = a.scale * kLog2e;
+  const uint32_t rowh = DROP ? row_hash(eff_seed(a), bh, myq) : 0u;
+  float m = -INFINITY, l = 0.f;  // running base-2 maximum (both halves agree), this half's sum
+  f16v O[DN];                    // O^T: dims 32 dn + acc_row(i) + 4h of query myq
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn) O[dn] = zero16();
+
+  int kbeg = 0, kend = nk;
+  if (a.causal) {
+    kend = min(nk, min(q0 + kTileQ, a.sq) + off);
+    kbeg = max(0, q0 + off - a.window + 1) & ~(kBlk - 1);
+  }
+  const int nb = kend > kbeg ? (kend - kbeg + kBlk - 1) / kBlk : 0;
+  const Stage<D, kBlk, 4> sk(a.k.st, a.hn, wave, lane), sv(a.v.st, a.hn, wave, lane);
+  const Frag<D> fr(lane);
+  auto stage = [&](int kb, char* buf) {
+    sk.issue(K + (int64_t)kb * a.k.st, a.k.st, a.hn, nk - kb, buf, wave);
+    sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, wave);
+  };
+  if (nb > 0) stage(kbeg, smem);
+  for (int ib = 0; ib < nb; ++ib) {
+    const int kb = kbeg + ib * kBlk;
+    const char* kimg = smem + (ib & 1) * 2 * IMG;
+    const char* vimg = kimg + IMG;
+    wait_vmcnt<0>();
+    lds_barrier();  // block ib is in LDS, block ib - 1 is read by every wave
+    if (ib + 1 < nb) stage(kb + kBlk, smem + ((ib + 1) & 1) * 2 * IMG);
+    if (q0w >= a.sq) continue;
+    if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
+    f16v S[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      S[t] = zero16();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) S[t] = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S[t]);
+    }
+    const bool diag = a.causal && kb + kBlk - 1 > q0w + off;
+    if (diag || kb + kBlk > nk) {
+      const int hi = (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) mask_hi(S[t], hi - 32 * t);
+    }
+    if (a.causal && kb < qlw + off - a.window + 1) {
+      const int lo = pos - a.window + 1 - kb - 4 * h;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) mask_lo(S[t], lo - 32 * t);
+    }
+    const float mx = half_max(fmaxf(tile_max(S[0]), tile_max(S[1]))) * c;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[dn][i] *= corr;
+      m = mn;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[t][i], c, nm));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[t][i + 1], c, nm));
+        ls[(i >> 1) & 3] += p0 + p1;
+        if (DROP) {
+          const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
+          S[t][i] = (x & 0xffffu) < thresh ? p0 : 0.f;
+          S[t][i + 1] = (x >> 16) < thresh ? p1 : 0.f;
+        } else {
+          S[t][i] = p0;
+          S[t][i + 1] = p1;
+        }
+      }
+    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const i4v pb = pack8<T>(S[t], u);
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(fr.tr(vimg, 32 * t + 16 * u, dn), pb, O[dn]);
+      }
+  }
+  l = half_sum(l);
+  if (myq < a.sq) {
+    const float inv = l > 0.f ? (DROP ? kscale : 1.f) / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+    T* out = at<T>(a.o, b, head) + (int64_t)myq * a.o.st;
+#pragma unroll
+    for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * dn + 8 * q < a.hn)
+          store4<T>(out + 32 * dn + 8 * q + 4 * h, O[dn][4 * q] * inv, O[dn][4 * q + 1] * inv, O[dn][4 * q + 2] * inv,
+                    O[dn][4 * q + 3] * inv);
+    if (h == 0) a.lse[(int64_t)bh * a.sq + myq] = l == 0.f ? INFINITY : m + __log2f(l);
+  }
+}
+
+// ---- forward, keys split over waves and workgroups ---------------------------------------------------------
+// For grids that would leave the card empty (few queries: single tokens against a long cache). The 32 lanes of
+// a tile are packed rows of one key head -- all r query heads of its group x sq queries -- so a group's K / V
+// are read once; every wave walks its own 32-key blocks with its own LDS buffers (no barrier in the loop), the
+// four waves join through LDS and the splits through an fp32 workspace.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk,
+                                                          float* __restrict__ ws) {
+  constexpr int RB = 2 * D, IMG = 32 * RB, KS = D / 16, DN = D / 32, NP = IMG / 1024;
+  constexpr int OS = D + 4;  // floats of a joined row: 4 of padding keep the 32 rows off one bank
+  __shared__ __attribute__((aligned(16))) char smem[4 * 4 * IMG > 4 * 32 * OS * 4 ? 4 * 4 * IMG : 4 * 32 * OS * 4];
+  __shared__ float sml[2][4][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int r = a.np / a.ng, rows = r * a.sq;
+  // problems (units x row tiles) fastest: the splits of a unit are spread in time, not over XCDs
+  const int units = a.b * a.ng, prob = blockIdx.x % (units * rtiles), split = blockIdx.x / (units * rtiles);
+  const int unit = prob % units, rt = prob / units;
+  const int b = unit / a.ng, g = unit % a.ng;
+  const int nk = seq_keys(a, b), off = a.sk - a.sq;
+  const int myr = rt * 32 + r32, jq = min(myr, rows - 1);
+  const int j = jq / a.sq, i_q = jq - j * a.sq, pos = i_q + off;
+  const T* K = at<const T>(a.k, b, g);
+  const T* V = at<const T>(a.v, b, g);
+  const T* Q = at<const T>(a.q, b, g * r) + (int64_t)j * a.q.sh;
+  i4v qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = load_frag<T>(Q, a.q.st, i_q, a.sq, 16 * s + 8 * h, a.hn);
+  const float c = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f16v O[DN];
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn) O[dn] = zero16();
+
+  const int k0 = split * chunk, k1 = min(nk, k0 + chunk);
+  // keys that some row of the tile sees (rows are query-major inside a head: any query may be in the tile)
+  char* mine = smem + wave * 4 * IMG;
+  const Stage<D, 32, 1> sk(a.k.st, a.hn, 0, lane), sv(a.v.st, a.hn, 0, lane);
+  const Frag<D> fr(lane);
+  auto stage = [&](int kb, char* buf) {
+    sk.issue(K + (int64_t)kb * a.k.st, a.k.st, a.hn, nk - kb, buf, 0);
+    sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, 0);
+  };
+  const int first = k0 + wave * 32;
+  if (first < k1) stage(first, mine);
+  int cur = 0;
+  for (int kb = first; kb < k1; kb += 128, cur ^= 1) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave is done with the other buffer
+    if (kb + 128 < k1) {
+      stage(kb + 128, mine + (cur ^ 1) * 2 * IMG);
+      wait_vmcnt<2 * NP>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    const char* kimg = mine + cur * 2 * IMG;
+    const char* vimg = kimg + IMG;
+    f16v S = zero16();
+#pragma unroll
+    for (int s = 0; s < KS; ++s) S = Mfma<T>::run(fr.row(kimg, 0, s), qf[s], S);
+    mask_hi(S, (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h);
+    if (a.causal) mask_lo(S, pos - a.window + 1 - kb - 4 * h);
+    const float mx = half_max(tile_max(S)) * c;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[dn][i] *= corr;
+      m = mn;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], c, nm));
+      l += S[i];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const i4v pb = pack8<T>(S, u);
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(fr.tr(vimg, 16 * u, dn), pb, O[dn]);
+    }
+  }
+  l = half_sum(l);
+  lds_barrier();  // every wave is done with its buffers: the same LDS now joins them
+  float* jo = reinterpret_cast<float*>(smem);
+  if (h == 0) {
+    sml[0][wave][r32] = m;
+    sml[1][wave][r32] = l;
+  }
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<f4v*>(jo + (wave * 32 + r32) * OS + 32 * dn + 8 * q + 4 * h) =
+          f4v{O[dn][4 * q], O[dn][4 * q + 1], O[dn][4 * q + 2], O[dn][4 * q + 3]};
+  __syncthreads();
+  constexpr int PER = D / 8;  // dims of a thread: 8 threads a row
+  const int row = tid >> 3, d0 = (tid & 7) * PER, grow = rt * 32 + row;
+  if (grow >= rows) return;
+  float mm = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[0][w][row]);
+  float lw = 0.f, acc[PER];
+#pragma unroll
+  for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float mw = sml[0][w][row], f = mw == -INFINITY ? (sml[1][w][row] == 0.f ? 0.f : 1.f)
+                                                         : __builtin_amdgcn_exp2f(mw - mm);
+    lw += f * sml[1][w][row];
+#pragma unroll
+    for (int d = 0; d < PER; ++d) acc[d] += f * jo[(w * 32 + row) * OS + d0 + d];
+  }
+  if (splits > 1) {
+    const int64_t slot = ((int64_t)prob * splits + split) * 32 + row;
+    float* wo = ws + slot * D + d0;
+#pragma unroll
+    for (int d = 0; d < PER; d += 4) *reinterpret_cast<f4v*>(wo + d) = f4v{acc[d], acc[d + 1], acc[d + 2], acc[d + 3]};
+    float* wm = ws + (int64_t)units * rtiles * splits * 32 * D + slot * 2;
+    if (d0 == 0) {
+      wm[0] = mm;
+      wm[1] = lw;
+    }
+    return;
+  }
+  const int jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
+  const float inv = lw > 0.f ? 1.f / lw : (lw == 0.f ? 0.f : lw);
+  T* out = at<T>(a.o, b, head) + (int64_t)iq * a.o.st;
+#pragma unroll
+  for (int d = 0; d < PER; d += 4)
+    if (d0 + d < a.hn) store4<T>(out + d0 + d, acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+  if (d0 == 0) a.lse[((int64_t)b * a.np + head) * a.sq + iq] = lw == 0.f ? INFINITY : mm + __log2f(lw);
+}
+
+// joins the splits: D / 4 threads a row, 4 dims each
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void k_ga_join(GaArgs a, int rtiles, int splits, const float* __restrict__ ws) {
+  constexpr int TPR = D / 4, RPB = kThreads / TPR;
+  const int r = a.np / a.ng, rows = r * a.sq, units = a.b * a.ng;
+  const int64_t id = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int d = (threadIdx.x % TPR) * 4;
+  const int prob = (int)(id / 32), row = (int)(id % 32);
+  if (prob >= units * rtiles) return;
+  const int unit = prob % units, grow = prob / units * 32 + row;
+  if (grow >= rows) return;
+  const float* wo = ws + ((int64_t)prob * splits * 32 + row) * D + d;
+  const float* wm = ws + (int64_t)units * rtiles * splits * 32 * D + ((int64_t)prob * splits * 32 + row) * 2;
+  float mm = -INFINITY;
+  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, wm[(int64_t)s * 64]);
+  float l = 0.f;
+  f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float ms = wm[(int64_t)s * 64], ls = wm[(int64_t)s * 64 + 1];
+    const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms - mm);
+    l += f * ls;
+    const f4v o = *reinterpret_cast<const f4v*>(wo + (int64_t)s * 32 * D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += f * o[i];
+  }
+  const int b = unit / a.ng, g = unit % a.ng, jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (d < a.hn)
+    store4<T>(at<T>(a.o, b, head) + (int64_t)iq * a.o.st + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  if (d == 0) a.lse[((int64_t)b * a.np + head) * a.sq + iq] = l == 0.f ? INFINITY : mm + __log2f(l);
+}
+
+// ---- backward --------------------------------------------------------------------------------------------
+// delta = rowsum(dO * O), 16 lanes a row of up to 128 values; with dropout also the row hashes
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ga_delta(GaArgs a) {
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 16;  // (b * np + head) * sq + q
+  const int sub = threadIdx.x & 15;
+  if (row >= (int64_t)a.b * a.np * a.sq) return;
+  const int bh = (int)(row / a.sq), q = (int)(row - (int64_t)bh * a.sq), b = bh / a.np, head = bh % a.np;
+  float acc = 0.f;
+  if (8 * sub < a.hn) {
+    float o[8], d[8];
+    VecIO<T>::load(at<const T>(a.o, b, head) + (int64_t)q * a.o.st + 8 * sub, o);
+    VecIO<T>::load(at<const T>(a.dout, b, head) + (int64_t)q * a.dout.st + 8 * sub, d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc = fmaf(o[i], d[i], acc);
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) acc += __shfl_xor(acc, s);
+  if (sub == 0) {
+    a.delta[row] = acc;
+    if (a.rowh) a.rowh[row] = row_hash(eff_seed(a), bh, q);
+  }
+}
+
+// dQ: the forward's layout. S^T = K Q^T and dP^T = V dO^T from row fragments, dS^T stays in registers and feeds
+// dQ^T = K^T dS^T (K^T by transposed reads of the same image).
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_t thresh, float kscale) {
+  constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
+  __shared__ __attribute__((aligned(16))) char smem[4 * IMG];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int r = a.np / a.ng;
+  Problem pr = problem(nx, a.b * a.ng, r, a.causal);
+  if (a.causal) pr.tile = nx - 1 - pr.tile;
+  const int b = pr.unit / a.ng, g = pr.unit % a.ng, head = g * r + pr.j, bh = b * a.np + head;
+  const int nk = seq_keys(a, b), off = a.sk - a.sq;
+  const int q0 = pr.tile * kTileQ, q0w = q0 + wave * 32, myq = q0w + r32, pos = myq + off;
+  const int qlw = min(q0w + 31, a.sq - 1);
+  const T* K = at<const T>(a.k, b, g);
+  const T* V = at<const T>(a.v, b, g);
+  i4v qf[KS], df[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    qf[s] = load_frag<T>(at<const T>(a.q, b, head), a.q.st, myq, a.sq, 16 * s + 8 * h, a.hn);
+    df[s] = load_frag<T>(at<const T>(a.dout, b, head), a.dout.st, myq, a.sq, 16 * s + 8 * h, a.hn);
+  }
+  const float c = a.scale * kLog2e;
+  const int64_t row = (int64_t)bh * a.sq + min(myq, a.sq - 1);
+  const float nl = -a.lse[row], dl = a.delta[row];
+  const uint32_t rowh = DROP ? a.rowh[row] : 0u;
+  f16v acc[DN];
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn) acc[dn] = zero16();
+  int kbeg = 0, kend = nk;
+  if (a.causal) {
+    kend = min(nk, min(q0 + kTileQ, a.sq) + off);
+    kbeg = max(0, q0 + off - a.window + 1) & ~(kBlk - 1);
+  }
+  const int nb = kend > kbeg ? (kend - kbeg + kBlk - 1) / kBlk : 0;
+  const Stage<D, kBlk, 4> sk(a.k.st, a.hn, wave, lane), sv(a.v.st, a.hn, wave, lane);
+  const Frag<D> fr(lane);
+  auto stage = [&](int kb, char* buf) {
+    sk.issue(K + (int64_t)kb * a.k.st, a.k.st, a.hn, nk - kb, buf, wave);
+    sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, wave);
+  };
+  if (nb > 0) stage(kbeg, smem);
+  for (int ib = 0; ib < nb; ++ib) {
+    const int kb = kbeg + ib * kBlk;
+    const char* kimg = smem + (ib & 1) * 2 * IMG;
+    const char* vimg = kimg + IMG;
+    wait_vmcnt<0>();
+    lds_barrier();
+    if (ib + 1 < nb) stage(kb + kBlk, smem + ((ib + 1) & 1) * 2 * IMG);
+    if (q0w >= a.sq) continue;
+    if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
+    const bool mh = (a.causal && kb + kBlk - 1 > q0w + off) || kb + kBlk > nk;
+    const bool ml = a.causal && kb < qlw + off - a.window + 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f16v S = zero16(), P = zero16();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        S = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S);
+        P = Mfma<T>::run(fr.row(vimg, 32 * t, s), df[s], P);  // dP^T
+      }
+      if (mh) mask_hi(S, (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h - 32 * t);
+      if (ml) mask_lo(S, pos - a.window + 1 - kb - 4 * h - 32 * t);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i], c, nl));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], c, nl));
+        if (DROP) {
+          const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
+          P[i] = p0 * (((x & 0xffffu) < thresh ? P[i] * kscale : 0.f) - dl);
+          P[i + 1] = p1 * (((x >> 16) < thresh ? P[i + 1] * kscale : 0.f) - dl);
+        } else {
+          P[i] = p0 * (P[i] - dl);
+          P[i + 1] = p1 * (P[i + 1] - dl);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const i4v sb = pack8<T>(P, u);
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn) acc[dn] = Mfma<T>::run(fr.tr(kimg, 32 * t + 16 * u, dn), sb, acc[dn]);
+      }
+    }
+  }
+  if (myq < a.sq) {
+    T* dq = at<T>(a.dq, b, head) + (int64_t)myq * a.dq.st;
+#pragma unroll
+    for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * dn + 8 * q < a.hn)
+          store4<T>(dq + 32 * dn + 8 * q + 4 * h, acc[dn][4 * q] * a.scale, acc[dn][4 * q + 1] * a.scale,
+                    acc[dn][4 * q + 2] * a.scale, acc[dn][4 * q + 3] * a.scale);
+  }
+}
+
+// dK / dV: workgroup = 4 waves x 32 keys of one key head, the key on the lane; it walks the 64-query blocks of
+// all r query heads of the group, so the gradients of shared heads are summed in the accumulators (no atomics,
+// one order). S = Q K^T and dP = dO V^T from row fragments (K / V stay in registers), P and dS feed
+// dV^T = dO^T P and dK^T = Q^T dS from the accumulators. -L, delta and the row hashes of the block ride along.
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, uint32_t thresh, float kscale) {
+  constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32, BUF = 2 * IMG + 3 * 256;
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  const int r = a.np / a.ng;
+  const Problem pr = problem(nx, a.b * a.ng, 1, a.causal);
+  const int b = pr.unit / a.ng, g = pr.unit % a.ng;
+  const int nk = seq_keys(a, b), off = a.sk - a.sq;
+  const int k0 = pr.tile * kTileQ, k0w = k0 + wave * 32, mykey = k0w + r32;
+  i4v kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    kf[s] = load_frag<T>(at<const T>(a.k, b, g), a.k.st, mykey, nk, 16 * s + 8 * h, a.hn);
+    vf[s] = load_frag<T>(at<const T>(a.v, b, g), a.v.st, mykey, nk, 16 * s + 8 * h, a.hn);
+  }
+  const float c = a.scale * kLog2e;
+  f16v dK[DN], dV[DN];
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn) dK[dn] = dV[dn] = zero16();
+  // queries that see a key of the tile: key - off <= i < key - off + window
+  int qbeg = 0, qend = k0 < nk ? a.sq : 0;
+  if (a.causal) {
+    qbeg = max(0, k0 - off) & ~(kBlk - 1);
+    qend = min(qend, min(k0 + kTileQ, nk) - 1 - off + a.window);
+  }
+  const int nqb = qend > qbeg ? (qend - qbeg + kBlk - 1) / kBlk : 0, total = nqb * r;
+  const Stage<D, kBlk, 4> sq(a.q.st, a.hn, wave, lane), sd(a.dout.st, a.hn, wave, lane);
+  const Frag<D> fr(lane);
+  auto stage = [&](int it, char* buf) {
+    const int j = it / nqb, q0 = qbeg + (it - j * nqb) * kBlk, head = g * r + j;
+    sq.issue(at<const T>(a.q, b, head) + (int64_t)q0 * a.q.st, a.q.st, a.hn, a.sq - q0, buf, wave);
+    sd.issue(at<const T>(a.dout, b, head) + (int64_t)q0 * a.dout.st, a.dout.st, a.hn, a.sq - q0, buf + IMG, wave);
+    // rows past the last query read as zeros: their Q and dO rows are zero too, so P = 1 meets dO = 0
+    const int64_t row = ((int64_t)b * a.np + head) * a.sq + q0;
+    const uint32_t bytes = 4u * (uint32_t)min(a.sq - q0, kBlk);
+    const unsigned l = __builtin_amdgcn_readfirstlane(lds_addr(buf + 2 * IMG));
+    if (wave == 0) dma4(make_rsrc(a.lse + row, bytes), lane * 4, l);
+    else if (wave == 1) dma4(make_rsrc(a.delta + row, bytes), lane * 4, l + 256);
+    else if (DROP && wave == 2) dma4(make_rsrc(a.rowh + row, bytes), lane * 4, l + 512);
+  };
+  if (total > 0) stage(0, smem);
+  for (int it = 0; it < total; ++it) {
+    const int j = it / nqb, q0 = qbeg + (it - j * nqb) * kBlk;
+    const char* qimg = smem + (it & 1) * BUF;
+    const char* dimg = qimg + IMG;
+    const float* lp = reinterpret_cast<const float*>(dimg + IMG);
+    wait_vmcnt<0>();
+    lds_barrier();
+    if (it + 1 < total) stage(it + 1, smem + ((it + 1) & 1) * BUF);
+    if (k0w >= nk) continue;
+    if (a.causal && (q0 + kBlk - 1 + off < k0w || q0 + off - a.window + 1 > k0w + 31)) continue;
+    const bool ml = a.causal && q0 + off < k0w + 31;                             // some query precedes some key
+    const bool mh = a.causal && q0 + kBlk - 1 + off - a.window + 1 > k0w;        // some key left the window
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f16v S = zero16(), P = zero16();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        S = Mfma<T>::run(fr.row(qimg, 32 * t, s), kf[s], S);
+        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), vf[s], P);  // dP
+      }
+      if (ml) mask_lo(S, mykey - off - q0 - 4 * h - 32 * t);
+      if (mh) mask_hi(S, mykey - off + a.window - 1 - q0 - 4 * h - 32 * t);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float* at4 = lp + 32 * t + 8 * q + 4 * h;
+        const f4v l4 = *reinterpret_cast<const f4v*>(at4), d4 = *reinterpret_cast<const f4v*>(at4 + 64);
+        i4v r4 = i4v{0, 0, 0, 0};
+        if (DROP) r4 = *reinterpret_cast<const i4v*>(at4 + 128);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * q + e;
+          const float p = __builtin_amdgcn_exp2f(fmaf(S[i], c, -l4[e]));
+          if (DROP) {
+            const uint32_t x = pair_hash((uint32_t)r4[e], mykey);
+            const float kk = ((mykey & 1) ? (x >> 16) : (x & 0xffffu)) < thresh ? kscale : 0.f;
+            S[i] = p * kk;
+            P[i] = p * (P[i] * kk - d4[e]);
+          } else {
+            S[i] = p;
+            P[i] = p * (P[i] - d4[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const i4v pb = pack8<T>(S, u), sb = pack8<T>(P, u);
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn) {
+          dV[dn] = Mfma<T>::run(fr.tr(dimg, 32 * t + 16 * u, dn), pb, dV[dn]);
+          dK[dn] = Mfma<T>::run(fr.tr(qimg, 32 * t + 16 * u, dn), sb, dK[dn]);
+        }
+      }
+    }
+  }
+  if (mykey < a.sk) {  // keys past the sequence's length take zeros, whatever their lanes held
+    const bool real = mykey < nk;
+    T* dk = at<T>(a.dk, b, g) + (int64_t)mykey * a.dk.st;
+    T* dv = at<T>(a.dv, b, g) + (int64_t)mykey * a.dv.st;
+#pragma unroll
+    for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * dn + 8 * q < a.hn) {
+          float x[4], y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = real ? dK[dn][4 * q + e] * a.scale : 0.f;
+            y[e] = real ? dV[dn][4 * q + e] : 0.f;
+          }
+          store4<T>(dk + 32 * dn + 8 * q + 4 * h, x[0], x[1], x[2], x[3]);
+          store4<T>(dv + 32 * dn + 8 * q + 4 * h, y[0], y[1], y[2], y[3]);
+        }
+  }
+}
+
+inline void check_launch(const char* what) {
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
+}
+template <typename T> struct TypeTag { using type = T; };
+template <typename F> void dispatch(int dt, int hn, bool drop, F&& f) {
+  auto by_d = [&](auto t) {
+    auto by_drop = [&](auto d) {
+      if (drop) f(t, d, std::true_type{});
+      else f(t, d, std::false_type{});
+    };
+    if (hn <= 64) by_drop(std::integral_constant<int, 64>{});
+    else by_drop(std::integral_constant<int, 128>{});
+  };
+  switch (dt) {
+    case kF16: by_d(TypeTag<f16>{}); break;
+    case kBF16: by_d(TypeTag<bf16>{}); break;
+    default: throw std::runtime_error("grouped attention: fp16 / bf16 only");
+  }
+}
+// keep where a 16-bit hash is below this: floor((1 - p) 2^16)
+uint32_t keep_thresh(const GaArgs& a) { return (uint32_t)std::min(65536.0, (1.0 - (double)a.p_drop) * 65536.0); }
+float keep_scale(const GaArgs& a) { return a.p_drop < 1.f ? 1.f / (1.f - a.p_drop) : 0.f; }
+
+struct SplitPlan {
+  int rtiles = 0, splits = 0, chunk = 0;  // splits == 0: the tiled forward
+};
+SplitPlan split_plan(const GaArgs& a) {
+  SplitPlan p;
+  const int64_t tiled = (int64_t)((a.sq + kTileQ - 1) / kTileQ) * a.b * a.np;
+  if (a.p_drop > 0.f || tiled >= 256) return p;
+  const int64_t rows = (int64_t)(a.np / a.ng) * a.sq, rt = (rows + 31) / 32, probs = rt * a.b * a.ng;
+  const int64_t want = std::max<int64_t>(1, 256 / probs), most = std::max(1, (a.sk + 127) / 128);
+  const int64_t s = std::min(want, most);
+  p.rtiles = (int)rt;
+  p.chunk = (int)((((int64_t)a.sk + s - 1) / s + 127) / 128 * 128);
+  p.splits = (int)(((int64_t)a.sk + p.chunk - 1) / p.chunk);
+  return p;
+}
+
+}  // namespace
+
+int64_t ga_forward_workspace(const GaArgs& a) {
+  const SplitPlan p = split_plan(a);
+  if (p.splits <= 1) return 0;
+  const int64_t d = a.hn <= 64 ? 64 : 128;
+  return (int64_t)a.b * a.ng * p.rtiles * p.splits * 32 * (d + 2);
+}
+
+void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
+  const SplitPlan p = split_plan(a);
+  const int nx = (a.sq + kTileQ - 1) / kTileQ;
+  dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
+    using T = typename decltype(t)::type;
+    constexpr int D = decltype(dd)::value;
+    constexpr bool DROP = decltype(drop)::value;
+    if (p.splits > 0) {
+      if constexpr (!DROP) {
+        const int64_t probs = (int64_t)a.b * a.ng * p.rtiles;
+        hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(kThreads), 0, st, a, p.rtiles,
+                           p.splits, p.chunk, ws);
+        if (p.splits > 1) {
+          constexpr int rpb = kThreads / (D / 4);
+          hipLaunchKernelGGL((k_ga_join<T, D>), dim3((unsigned)((probs * 32 + rpb - 1) / rpb)), dim3(kThreads), 0, st,
+                             a, p.rtiles, p.splits, ws);
+        }
+      }
+    } else {
+      hipLaunchKernelGGL((k_ga_fwd<T, D, DROP>), dim3((unsigned)((int64_t)nx * a.b * a.np)), dim3(kThreads), 0, st, a,
+                         nx, keep_thresh(a), keep_scale(a));
+    }
+  });
+  check_launch("ga_forward");
+}
+
+void ga_backward(int dt, const GaArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.b * a.np * a.sq;
+  const dim3 gd((unsigned)((rows * 16 + kThreads - 1) / kThreads));
+  const int nq = (a.sq + kTileQ - 1) / kTileQ, nkt = (a.sk + kTileQ - 1) / kTileQ;
+  dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
+    using T = typename decltype(t)::type;
+    constexpr int D = decltype(dd)::value;
+    constexpr bool DROP = decltype(drop)::value;
+    hipLaunchKernelGGL((k_ga_delta<T>), gd, dim3(kThreads), 0, st, a);
+    if (a.dk.p)
+      hipLaunchKernelGGL((k_ga_dkdv<T, D, DROP>), dim3((unsigned)((int64_t)nkt * a.b * a.ng)), dim3(kThreads), 0, st, a,
+                         nkt, keep_thresh(a), keep_scale(a));
+    if (a.dq.p)
+      hipLaunchKernelGGL((k_ga_dq<T, D, DROP>), dim3((unsigned)((int64_t)nq * a.b * a.np)), dim3(kThreads), 0, st, a,
+                         nq, keep_thresh(a), keep_scale(a));
+  });
+  check_launch("ga_backward");
+}
+
+}  // namespace bh

@@ -1,0 +1,360 @@
+"""Grouped-query attention (transformer.functional.fused_grouped_attention, kernels/grouped_attn.hip) against its
+definition in fp64, with bounds computed beside it.
+
+Bounds, with u = half a step of the tensors' type (torch.finfo(t).eps / 2). The kernels round P (dropped) and dS to the
+type, everything else is fp32. e bounds the relative error of a probability: its score is a sum of hn products in
+fp32 (error (hn + 16) 2^-24 sum |scale q k|), the exponential, the fma in front of it and L add 2^-19.
+fp16 holds P below 2^-14 and dS below it only to 2^-25 (d below); bf16 has no such floor here.
+  |dO|   <= u |O| + sum_k (u + e) Pd |v| + d sum |v|
+  |ddelta| <= sum_d |dO| E_O,   |E_dS| <= P (ddelta + (e + 2^-19) (|dP| + |delta|)) + u |dS| + d
+  |dQ|   <= u |dQ| + scale sum_k E_dS |k|,   |dK| <= u |dK| + scale sum_q E_dS |q|
+  |dV|   <= u |dV| + sum_q (u + e) Pd |dO| + d sum |dO|
+and a sum of n fp32 terms adds n 2^-24 of its absolute terms (n = sk or r sq, folded into e)."""
+import math
+
+import pytest
+import torch
+
+from beforeholiday_amd.transformer.functional import attention_dropout_keep, fused_grouped_attention
+
+F8 = torch.float64
+
+
+def oracle(q, k, v, dout=None, *, causal=False, window=None, lens=None, p=0.0, seed=0, scale=None, fp16=False, u=0.0):
+    """(value, bound) of the output and, with dout, of dq, dk, dv; all [s, b, h, d] fp64 on the CPU."""
+    q, k, v = (t.detach().to("cpu", F8) for t in (q, k, v))
+    sq, b, np_, hn = q.shape
+    sk, ng = k.size(0), k.size(2)
+    r = np_ // ng
+    scale = hn ** -0.5 if scale is None else scale
+    qh = q.permute(1, 2, 0, 3)
+    kh, vh = (t.permute(1, 2, 0, 3).repeat_interleave(r, 1) for t in (k, v))
+    i = torch.arange(sq)[:, None] + sk - sq
+    j = torch.arange(sk)[None]
+    see = torch.ones(sq, sk, dtype=torch.bool)
+    if causal:
+        see &= j <= i
+        if window is not None:
+            see &= j > i - window
+    see = see.expand(b, np_, sq, sk).clone()
+    if lens is not None:
+        gone = j >= lens.cpu().clamp(0, sk).view(-1, 1, 1, 1)
+        see &= ~gone
+        kh, vh = (t.masked_fill(gone.transpose(-1, -2), 0.0) for t in (kh, vh))
+    s = (qh @ kh.transpose(-1, -2)) * scale
+    s = s.masked_fill(~see, -math.inf)
+    m = s.amax(-1, keepdim=True) if sk else torch.full((b, np_, sq, 1), -math.inf, dtype=F8)
+    e = torch.exp(s - m.masked_fill(m == -math.inf, 0.0))
+    tot = e.sum(-1, keepdim=True)
+    P = e / tot.masked_fill(tot == 0, 1.0)
+    w = torch.ones_like(P)
+    if p > 0:
+        w = attention_dropout_keep(seed, b * np_, sq, sk, p).view(b, np_, sq, sk).to(F8) / (1 - p)
+    Pd = P * w
+    O = Pd @ vh
+    ab = (qh.abs() @ kh.abs().transpose(-1, -2)).amax() * scale if sk and sq else torch.zeros((), dtype=F8)
+    eps = float((hn + 16) * 2.0 ** -24 * ab + 2.0 ** -19 + max(sk, r * sq) * 2.0 ** -24)
+    d = 2.0 ** -25 if fp16 else 0.0
+    seef = see.to(F8)
+    EO = u * O.abs() + (u + eps) * (Pd @ vh.abs()) + d * (seef @ vh.abs()) / (1 - p) + 1e-30
+
+    def heads(t):  # [b, h, s, d] -> [s, b, h, d]
+        return t.permute(2, 0, 1, 3)
+
+    def groups(t):  # sum of the query heads of a group
+        return t.view(b, ng, r, sk, hn).sum(2).permute(2, 0, 1, 3)
+
+    res = [(heads(O), heads(EO))]
+    if dout is None:
+        return res
+    g = dout.detach().to("cpu", F8).permute(1, 2, 0, 3)
+    dP = (g @ vh.transpose(-1, -2)) * w
+    delta = (P * dP).sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    dd = (g.abs() * EO).sum(-1, keepdim=True) + eps * (g.abs() * O.abs()).sum(-1, keepdim=True)
+    absdP = (g.abs() @ vh.abs().transpose(-1, -2)) * w
+    EdS = P * (dd + (eps + 2.0 ** -19) * (absdP + delta.abs())) + u * dS.abs() + d * seef
+    dQ = scale * dS @ kh
+    EQ = u * dQ.abs() + scale * EdS @ kh.abs() + d
+    dK = scale * dS.transpose(-1, -2) @ qh
+    EK = groups(scale * EdS.transpose(-1, -2) @ qh.abs())
+    dV = Pd.transpose(-1, -2) @ g
+    EV = groups((u + eps) * Pd.transpose(-1, -2) @ g.abs() + d * seef.transpose(-1, -2) @ g.abs() / (1 - p))
+    dK, dV = groups(dK), groups(dV)
+    return res + [(heads(dQ), heads(EQ) + 1e-30), (dK, EK + u * dK.abs() + d + 1e-30), (dV, EV + u * dV.abs() + d + 1e-30)]
+
+
+def within(got, want, bound, what):
+    got = got.detach().to("cpu", F8)
+    assert got.shape == want.shape, what
+    over = (got - want).abs() - bound
+    assert not torch.isnan(got).any(), what
+    assert (over <= 0).all(), f"{what}: {float((got - want).abs().max()):.3g} off, over its bound by {float(over.max()):.3g}"
+
+
+def make(sq, sk, b, np_, ng, hn, dtype, device, seed=0, layout="fused"):
+    g = torch.Generator().manual_seed(seed)
+    if layout == "fused" and sq == sk:
+        mixed = torch.randn(sq, b, (np_ + 2 * ng) * hn, generator=g).to(dtype).to(device)
+        q = mixed[..., :np_ * hn].view(sq, b, np_, hn)
+        k = mixed[..., np_ * hn:(np_ + ng) * hn].view(sk, b, ng, hn)
+        v = mixed[..., (np_ + ng) * hn:].view(sk, b, ng, hn)
+    else:
+        q, k, v = (torch.randn(s, b, h, hn, generator=g).to(dtype).to(device) for s, h in ((sq, np_), (sk, ng), (sk, ng)))
+    dout = torch.randn(sq, b, np_, hn, generator=g).to(dtype).to(device)
+    return tuple(t.detach().requires_grad_() for t in (q, k, v)) + (dout,)
+
+
+def check(sq, sk, b, np_, ng, hn, dtype, device="cuda", seed=0, lens=None, p=0.0, layout="fused", **kw):
+    q, k, v, dout = make(sq, sk, b, np_, ng, hn, dtype, device, seed, layout)
+    if lens is not None:
+        lens = torch.tensor(lens, dtype=torch.int32, device=device)
+    out = fused_grouped_attention(q, k, v, key_lengths=lens, dropout_p=p, seed=1234567891011 if p else None, **kw)
+    got = (out, *torch.autograd.grad(out, (q, k, v), dout))
+    want = oracle(q, k, v, dout, lens=lens, p=p, seed=1234567891011, fp16=dtype == torch.float16,
+                  u=torch.finfo(dtype).eps / 2 if dtype != F8 else 1e-12, **kw)
+    for name, g, (w, e) in zip(("out", "dq", "dk", "dv"), got, want):
+        within(g, w, e, name)
+    with torch.no_grad():  # the call without a graph takes the same kernels
+        assert torch.equal(fused_grouped_attention(q, k, v, key_lengths=lens, dropout_p=p,
+                                                   seed=1234567891011 if p else None, **kw), out)
+
+
+SHAPES = [(1, 1, 1, 1, 1, 8), (5, 5, 2, 4, 2, 16), (33, 33, 2, 6, 2, 40), (64, 64, 1, 8, 8, 64), (7, 70, 2, 4, 1, 24),
+          (70, 7, 1, 2, 2, 32)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("kw", [{}, {"causal": True}, {"causal": True, "window": 5}, {"p": 0.3, "causal": True}])
+def test_cpu_path_is_the_definition(shape, kw):
+    check(*shape, F8, "cpu", **kw)
+
+
+def test_cpu_key_lengths_and_garbage_past_them():
+    q, k, v, _ = make(6, 9, 3, 4, 2, 16, torch.float32, "cpu")
+    lens = torch.tensor([9, 0, 4])
+    want = fused_grouped_attention(q, k, v, key_lengths=lens)
+    k2, v2 = k.detach().clone(), v.detach().clone()
+    k2[4:, 2], v2[4:, 2] = float("nan"), float("inf")
+    got = fused_grouped_attention(q, k2, v2, key_lengths=lens)
+    assert torch.equal(got, want) and (got[:, 1] == 0).all()
+
+
+def test_cpu_gradients_against_differences():
+    q, k, v, dout = make(5, 7, 2, 4, 2, 8, F8, "cpu")
+    lens = torch.tensor([7, 3])
+    f = lambda *t: fused_grouped_attention(*t, causal=True, window=4, key_lengths=lens)  # noqa: E731
+    assert torch.autograd.gradcheck(f, (q, k, v), eps=1e-6, atol=1e-7)
+
+
+@pytest.mark.parametrize("bad, kw", [
+    (lambda q, k, v: (q[0], k, v), {}),
+    (lambda q, k, v: (q, k[:3], v), {}),
+    (lambda q, k, v: (q[:, :1], k, v), {}),
+    (lambda q, k, v: (q[:, :, :3], k, v), {}),
+    (lambda q, k, v: (q[..., :8], k, v), {}),
+    (lambda q, k, v: (q, k[:, :, :0], v[:, :, :0]), {}),
+    (lambda q, k, v: (q, k.double(), v), {}),
+    (lambda q, k, v: (q, k, v), {"window": 4}),
+    (lambda q, k, v: (q, k, v), {"window": 0, "causal": True}),
+    (lambda q, k, v: (q, k, v), {"dropout_p": 1.0}),
+    (lambda q, k, v: (q, k, v), {"dropout_p": -0.1}),
+    (lambda q, k, v: (q, k, v), {"scale": 0.0}),
+    (lambda q, k, v: (q, k, v), {"scale": float("nan")}),
+    (lambda q, k, v: (q, k, v), {"key_lengths": torch.tensor([4])}),
+    (lambda q, k, v: (q, k, v), {"key_lengths": torch.tensor([4.0, 4.0])}),
+])
+def test_refusals(bad, kw):
+    q, k, v, _ = make(4, 4, 2, 4, 2, 16, torch.float32, "cpu")
+    with pytest.raises(ValueError):
+        fused_grouped_attention(*bad(q, k, v), **kw)
+
+
+def test_keep_flags_match_their_rate_and_differ_by_head_and_seed():
+    a = attention_dropout_keep(5, 4, 64, 64, 0.25)
+    assert abs(a.float().mean() - 0.75) < 0.02 and not torch.equal(a[0], a[1])
+    assert not torch.equal(a, attention_dropout_keep(6, 4, 64, 64, 0.25))
+    assert torch.equal(a[:, :, :31], attention_dropout_keep(5, 4, 64, 31, 0.25))
+
+
+# ---- GPU -----------------------------------------------------------------------------------------------------
+gpu = pytest.mark.gpu
+H16 = [torch.float16, torch.bfloat16]
+
+
+@gpu
+@pytest.mark.parametrize("bad", ["fp32", "hn", "lens_device", "lens_dtype"])
+def test_gpu_refusals(bad):
+    q, k, v, _ = make(4, 4, 2, 4, 2, 12 if bad == "hn" else 16, torch.float32 if bad == "fp32" else torch.float16, "cuda")
+    lens = {"lens_device": torch.tensor([1, 2]), "lens_dtype": torch.tensor([1.0, 2.0], device="cuda")}.get(bad)
+    with pytest.raises((ValueError, RuntimeError)):
+        fused_grouped_attention(q, k, v, key_lengths=lens)
+
+
+GPU_SHAPES = SHAPES + [(1, 300, 2, 8, 2, 128), (128, 128, 2, 4, 2, 128), (129, 129, 1, 3, 1, 80), (257, 257, 2, 8, 2, 64),
+                       (64, 515, 2, 4, 2, 96), (200, 63, 1, 4, 4, 128), (385, 640, 8, 16, 8, 128), (511, 511, 8, 16, 4, 56)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", H16)
+@pytest.mark.parametrize("shape", GPU_SHAPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_against_definition(shape, causal, dtype):
+    check(*shape, dtype, causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("window", [1, 31, 64, 100, 1000])
+@pytest.mark.parametrize("shape", [(300, 300, 2, 4, 2, 128), (300, 450, 8, 16, 8, 64), (3, 400, 1, 4, 1, 64)])
+def test_window(shape, window):
+    check(*shape, torch.bfloat16, causal=True, window=window)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(200, 200, 4, 4, 2, 128), (1, 700, 4, 8, 2, 128), (150, 150, 4, 64, 16, 40)])
+def test_key_lengths(shape, causal):
+    sk = shape[1]
+    check(*shape, torch.float16, causal=causal, lens=[sk, 0, 1, sk - 67])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", H16)
+@pytest.mark.parametrize("shape", [(200, 200, 2, 4, 2, 128), (65, 129, 1, 8, 8, 64), (1, 90, 2, 2, 1, 24)])
+@pytest.mark.parametrize("p", [0.1, 0.9])
+def test_dropout(shape, p, dtype):
+    check(*shape, dtype, p=p, causal=True)
+
+
+@gpu
+def test_garbage_past_key_lengths_is_not_read():
+    for shape in ((6, 200, 3, 4, 2, 64), (200, 200, 3, 128, 64, 128)):
+        q, k, v, dout = make(*shape, torch.bfloat16, "cuda")
+        lens = torch.tensor([shape[1], 0, 77], device="cuda")
+        out = fused_grouped_attention(q, k, v, key_lengths=lens)
+        want = (out, *torch.autograd.grad(out, (q, k, v), dout))
+        k2, v2 = k.detach().clone(), v.detach().clone()
+        k2[77:, 2], v2[77:, 2], k2[:, 1] = float("nan"), float("inf"), float("nan")
+        k2.requires_grad_(), v2.requires_grad_()
+        out = fused_grouped_attention(q, k2, v2, key_lengths=lens)
+        got = (out, *torch.autograd.grad(out, (q, k2, v2), dout))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert (got[0][:, 1] == 0).all() and (got[1][:, 1] == 0).all() and (got[2][77:, 2] == 0).all() and (got[3][77:, 2] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("value", [60000.0, -60000.0])
+def test_extreme_scores(value):
+    """One key far above (below) all others: the running maximum jumps by more than any deferral."""
+    q, k, v, dout = make(140, 140, 1, 2, 2, 64, torch.float16, "cuda")
+    with torch.no_grad():
+        k[70] = value / 64 * q.detach()[70].sign()
+    check_like = oracle(q, k, v, dout, fp16=True, u=torch.finfo(torch.float16).eps / 2)
+    out = fused_grouped_attention(q, k, v)
+    for name, g, (w, e) in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), dout)), check_like):
+        within(g, w, e, name)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["batch_first", "heads_first", "odd_stride", "not_contiguous", "expanded"])
+def test_layouts_agree(layout):
+    q, k, v, dout = (t.detach() for t in make(150, 150, 2, 4, 2, 64, torch.bfloat16, "cuda", layout="plain"))
+    want_in = [t.clone().requires_grad_() for t in (q, k, v)]
+    if layout == "expanded":  # one key / value for the whole batch, one position for all of them
+        want_in = [want_in[0]] + [t.detach()[:1, :1].expand(150, 2, 2, 64).clone().requires_grad_() for t in want_in[1:]]
+    out = fused_grouped_attention(*want_in, causal=True)
+    want = (out, *torch.autograd.grad(out, want_in, dout))
+
+    def view(t):
+        if layout == "batch_first":
+            return t.transpose(0, 1).contiguous().transpose(0, 1)
+        if layout == "heads_first":
+            return t.permute(1, 2, 0, 3).contiguous().permute(2, 0, 1, 3)
+        if layout == "odd_stride":
+            return torch.zeros(*t.shape[:3], 67, dtype=t.dtype, device=t.device)[..., 3:].copy_(t)
+        return t.transpose(2, 3).contiguous().transpose(2, 3)
+
+    if layout == "expanded":
+        got_in = [q.clone().requires_grad_()] + [t[:1, :1].expand(150, 2, 2, 64).detach().requires_grad_() for t in (k, v)]
+        assert got_in[1].stride()[:2] == (0, 0)
+    else:
+        got_in = [view(t).detach().requires_grad_() for t in (q, k, v)]
+        dout = view(dout)
+    out = fused_grouped_attention(*got_in, causal=True)
+    got = (out, *torch.autograd.grad(out, got_in, dout))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(0, 5, 2, 4, 2, 64), (5, 0, 2, 4, 2, 64), (5, 5, 0, 4, 2, 64)])
+def test_empty(shape):
+    q, k, v, dout = make(*shape, torch.float16, "cuda", layout="plain")
+    out = fused_grouped_attention(q, k, v, causal=True)
+    assert out.shape == q.shape and (out == 0).all()
+    for g in torch.autograd.grad(out, (q, k, v), dout):
+        assert (g == 0).all()
+
+
+@gpu
+def test_only_some_gradients_and_no_second_derivative():
+    q, k, v, dout = make(40, 40, 2, 4, 2, 64, torch.float16, "cuda", layout="plain")
+    out = fused_grouped_attention(q, k, v)
+    want = torch.autograd.grad(out, (q, k, v), dout)
+    for i in range(3):
+        t = [x.detach().requires_grad_(n == i) for n, x in enumerate((q, k, v))]
+        (g,) = torch.autograd.grad(fused_grouped_attention(*t), t[i], dout)
+        assert torch.equal(g, want[i])
+    q.requires_grad_()
+    (g,) = torch.autograd.grad(fused_grouped_attention(q, k, v).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@gpu
+def test_same_bits_again_and_on_another_stream():
+    q, k, v, dout = make(300, 300, 2, 8, 2, 128, torch.bfloat16, "cuda")
+    run = lambda: (lambda o: (o, *torch.autograd.grad(o, (q, k, v), dout)))(  # noqa: E731
+        fused_grouped_attention(q, k, v, causal=True, dropout_p=0.1, seed=3))
+    a, b = run(), run()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c = run()
+    torch.cuda.current_stream().wait_stream(s)
+    for x, y, z in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+@gpu
+def test_captured_and_replayed():
+    """Two captured calls (split keys with its workspace, and tiled) replay to the eager bits with new inputs between."""
+    shapes = [(2, 900, 2, 8, 2, 128), (300, 300, 4, 32, 8, 64)]
+    runs = []
+    for shape in shapes:
+        q, k, v, dout = make(*shape, torch.bfloat16, "cuda", layout="plain")
+
+        def step(q=q, k=k, v=v, dout=dout):
+            o = fused_grouped_attention(q, k, v, causal=True)
+            return (o, *torch.autograd.grad(o, (q, k, v), dout))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        runs.append((graph, outs, step, (q, k, v)))
+    for n in range(3):
+        for graph, outs, step, ins in runs:
+            with torch.no_grad():
+                for t in ins:
+                    t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(n)))
+        for graph, *_ in runs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, outs, step, ins in runs:
+            for a, b in zip(outs, step()):
+                assert torch.equal(a, b)

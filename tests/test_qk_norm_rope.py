@@ -1,0 +1,308 @@
+"""Query / key norm + rotary embedding (transformer.functional.fused_qk_norm_rope, kernels/qk_norm_rope.hip) against the
+definition in fp64.
+
+Bounds: all math is fp32 (each of the at most hn + 12 roundings on a value's path is half a step, 2^-24 of the absolute
+terms) and one rounding to the type, u = finfo.eps / 2 (plus 2^-25: fp16 below its normal range). A weight's gradient is a
+sum of n = s b heads terms: n 2^-24 of the absolute terms, the worst order, and the rounding to the weight's type."""
+import math
+
+import pytest
+import torch
+
+from beforeholiday_amd.transformer.functional import fused_qk_norm_rope, rotary_tables
+
+F8 = torch.float64
+
+
+def oracle(x, w, dy, cos, sin, pos, eps, inter, u):
+    """(y, dx, dw) of one operand as (value, bound), fp64 on the CPU; bounds before the final rounding are 2^-24 (hn + 12)
+    of the absolute terms."""
+    x = x.detach().to("cpu", F8)
+    hn = x.size(3)
+    e = (hn + 12) * 2.0 ** -24
+    n, r = x, None
+    if w is not None:
+        w = w.detach().to("cpu", F8)
+        r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+        n = x * r * w
+
+    def turn(t, sign, absolute=False):
+        if cos is None:
+            return t
+        c, s = (a.cpu().to(F8)[pos][:, :, None] for a in (cos, sin))
+        if absolute:
+            c, s, sign = c.abs(), s.abs(), -1  # |a||c| + |b||s| and |b||c| + |a||s| need one sign each
+        h = c.size(-1)
+        a, b = (t[..., 0:2 * h:2], t[..., 1:2 * h:2]) if inter else (t[..., :h], t[..., h:2 * h])
+        if absolute:
+            y, z = a * c + b * s, b * c + a * s
+        else:
+            y, z = a * c - sign * b * s, b * c + sign * a * s
+        out = t.clone()
+        if inter:
+            out[..., 0:2 * h:2], out[..., 1:2 * h:2] = y, z
+        else:
+            out[..., :h], out[..., h:2 * h] = y, z
+        return out
+
+    y = turn(n, 1)
+    res = {"y": (y, u * y.abs() + e * turn(n.abs(), 1, True) + 2.0 ** -25)}
+    if dy is None:
+        return res
+    g = dy.detach().to("cpu", F8)
+    dn, adn = turn(g, -1), turn(g.abs(), 1, True)
+    if w is None:
+        res["dx"] = (dn, u * dn.abs() + e * adn + 2.0 ** -25)
+        return res
+    xh = x * r
+    gw = dn * w
+    m = (gw * xh).mean(-1, keepdim=True)
+    am = (adn * w.abs() * xh.abs()).mean(-1, keepdim=True)
+    dx = r * (gw - xh * m)
+    res["dx"] = (dx, u * dx.abs() + 3 * e * r * (adn * w.abs() + xh.abs() * am) + 2.0 ** -25)
+    terms = x.size(0) * x.size(1) * x.size(2)
+    res["dw"] = ((dn * xh).sum((0, 1, 2)), (e + terms * 2.0 ** -24) * (adn * xh.abs()).sum((0, 1, 2)) + 1e-30)
+    return res
+
+
+def within(got, pair, what, extra=0.0):
+    want, bound = pair
+    got = got.detach().to("cpu", F8)
+    assert got.shape == want.shape and not torch.isnan(got).any(), what
+    over = (got - want).abs() - bound - extra * want.abs()
+    assert over.numel() == 0 or float(over.max()) <= 0, f"{what}: over its bound by {float(over.max()):.3g}"
+
+
+def check(s, b, np_, ng, hn, dtype, device="cuda", rot=None, norm=True, inter=False, pos=None, wdtype=torch.float32,
+          offset=0, layout="fused", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rot = hn if rot is None else rot
+    mixed = torch.randn(s, b, (np_ + ng) * hn + (5 if layout == "odd" else 0), generator=g).to(dtype).to(device)
+    if layout == "odd":
+        mixed = mixed[..., 5:]
+    q, k = mixed[..., :np_ * hn].view(s, b, np_, hn), mixed[..., np_ * hn:].view(s, b, ng, hn)
+    if layout == "transposed":
+        q, k = (t.permute(3, 1, 2, 0).contiguous().permute(3, 1, 2, 0) for t in (q, k))
+    q, k = q.detach().requires_grad_(), k.detach().requires_grad_()
+    wq, wk = ((1 + torch.randn(hn, generator=g)).to(wdtype).to(device).requires_grad_() for _ in range(2)) if norm else (None, None)
+    cos = sin = None
+    if rot:
+        cos, sin = rotary_tables(4096, rot, device=device)
+    where = None
+    if pos == "s":
+        where = torch.randint(4096, (s,), generator=g).to(device)
+    elif pos == "sb":
+        where = torch.randint(4096, (s, b), generator=g).to(torch.int32).to(device)
+    elif pos == "sb_t":
+        where = torch.randint(4096, (b, s), generator=g).to(device).t()
+    dq, dk = (torch.randn(t.shape, generator=g).to(dtype).to(device) for t in (q, k))
+    if layout == "transposed":
+        dq = dq.permute(3, 1, 2, 0).contiguous().permute(3, 1, 2, 0)
+    yq, yk = fused_qk_norm_rope(q, k, wq, wk, cos, sin, positions=where, offset=offset, interleaved=inter)
+    assert yq.is_contiguous() and yk.is_contiguous() and yq.dtype == dtype
+    leaves = (q, k) + ((wq, wk) if norm else ())
+    grads = torch.autograd.grad((yq, yk), leaves, (dq, dk))
+    row = torch.arange(offset, offset + s)[:, None].expand(s, b) if where is None else \
+        where.cpu().long() if where.dim() == 2 else where.cpu()[:, None].expand(s, b)
+    u = torch.finfo(dtype).eps / 2
+    for n, (x, w, y, dy, name) in enumerate(((q, wq, yq, dq, "query"), (k, wk, yk, dk, "key"))):
+        want = oracle(x, w, dy, cos, sin, row, 1e-6, inter, u)
+        within(y, want["y"], name)
+        within(grads[n], want["dx"], name + " gradient")
+        if norm:
+            within(grads[2 + n], want["dw"], name + " weight gradient", torch.finfo(wdtype).eps / 2 if wdtype != torch.float32 else 0.0)
+    with torch.no_grad():
+        for a, c in zip(fused_qk_norm_rope(q, k, wq, wk, cos, sin, positions=where, offset=offset, interleaved=inter), (yq, yk)):
+            assert torch.equal(a, c)
+
+
+SHAPES = [(1, 1, 1, 1, 2), (1, 5, 4, 2, 64), (7, 3, 6, 2, 80), (33, 2, 3, 1, 128), (5, 2, 2, 2, 34)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("norm, half", [(True, False), (False, True), (True, True)])
+def test_cpu_path_is_the_definition(shape, inter, norm, half):
+    check(*shape, torch.float32, "cpu", rot=(shape[4] // 4) * 2 if half and shape[4] > 2 else None, norm=norm, inter=inter)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_cpu_gradients_against_differences(inter):
+    g = torch.Generator().manual_seed(1)
+    q, k, wq, wk = (torch.randn(*s, generator=g, dtype=F8).requires_grad_() for s in ((3, 2, 2, 8), (3, 2, 1, 8), (8,), (8,)))
+    cos, sin = rotary_tables(16, 4)
+    pos = torch.tensor([[3, 0], [15, 2], [2, 2]])
+    f = lambda *t: fused_qk_norm_rope(*t, cos, sin, positions=pos, interleaved=inter)  # noqa: E731
+    assert torch.autograd.gradcheck(f, (q, k, wq, wk), eps=1e-6, atol=1e-7)
+
+
+def test_tables_keep_far_angles():
+    cos, sin = rotary_tables(200001, 4, base=100.0)
+    at = 200000 * 100.0 ** -0.5
+    assert abs(float(cos[200000, 0]) - math.cos(200000.0)) < 1e-7 and abs(float(sin[200000, 1]) - math.sin(at)) < 1e-7
+    assert torch.equal(rotary_tables(9, 4, position_scale=0.5)[0][8], rotary_tables(9, 4)[0][4])
+    with pytest.raises(ValueError):
+        rotary_tables(4, 3)
+
+
+@pytest.mark.parametrize("bad", ["dim", "shape", "one_weight", "one_table", "nothing", "weight_size", "table_wide", "table_dtype",
+                                 "pos_shape", "pos_dtype", "past_end", "offset_and_pos", "negative"])
+def test_refusals(bad):
+    q, k, w = torch.randn(4, 2, 4, 8), torch.randn(4, 2, 2, 8), torch.ones(8)
+    cos, sin = rotary_tables(6, 8)
+    pos = torch.zeros(4, 2, dtype=torch.int64)
+    args, kw = [q, k, w, w, cos, sin], {}
+    if bad == "dim":
+        args[0] = q[0]
+    elif bad == "shape":
+        args[1] = k[:3]
+    elif bad == "one_weight":
+        args[3] = None
+    elif bad == "one_table":
+        args[5] = None
+    elif bad == "nothing":
+        args[2:] = [None] * 4
+    elif bad == "weight_size":
+        args[2] = torch.ones(6)
+    elif bad == "table_wide":
+        args[4:] = rotary_tables(6, 10)
+    elif bad == "table_dtype":
+        args[4:] = [cos.double(), sin.double()]
+    elif bad == "pos_shape":
+        kw = {"positions": pos.t()}
+    elif bad == "pos_dtype":
+        kw = {"positions": pos.float()}
+    elif bad == "past_end":
+        kw = {"offset": 3}
+    elif bad == "offset_and_pos":
+        kw = {"positions": pos, "offset": 1}
+    elif bad == "negative":
+        kw = {"offset": -1}
+    with pytest.raises(ValueError):
+        fused_qk_norm_rope(*args, **kw)
+
+
+def test_cpu_position_outside_the_tables_gives_nan():
+    q, k = torch.randn(3, 1, 1, 8), torch.randn(3, 1, 1, 8)
+    y, _ = fused_qk_norm_rope(q, k, None, None, *rotary_tables(4, 4), positions=torch.tensor([0, 4, -1]))
+    assert torch.isnan(y[1:, ..., :4]).all() and torch.equal(y[1:, ..., 4:], q[1:, ..., 4:]) and not torch.isnan(y[0]).any()
+
+
+# ---- GPU -----------------------------------------------------------------------------------------------------
+gpu = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+GPU_SHAPES = SHAPES + [(1, 64, 32, 8, 128), (257, 3, 5, 1, 96), (700, 4, 16, 16, 64), (40, 2, 3, 3, 256), (9, 2, 2, 1, 512)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", GPU_SHAPES)
+@pytest.mark.parametrize("inter", [False, True])
+def test_against_definition(shape, inter, dtype):
+    check(*shape, dtype, inter=inter)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("rot", [0, 2, 16, 20, 40, 80])
+def test_partial_rotation_and_norm_alone(rot, inter, dtype):
+    check(21, 3, 6, 2, 80, dtype, rot=rot, inter=inter)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotation_alone(inter, dtype):
+    check(65, 2, 4, 2, 64, dtype, norm=False, inter=inter)
+
+
+@gpu
+@pytest.mark.parametrize("pos", ["s", "sb", "sb_t"])
+def test_positions(pos):
+    check(31, 5, 4, 2, 64, torch.bfloat16, pos=pos)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["odd", "transposed"])
+@pytest.mark.parametrize("wdtype", TYPES)
+def test_layouts_weight_types_and_offset(layout, wdtype):
+    check(19, 4, 4, 2, 64, torch.bfloat16, layout=layout, wdtype=wdtype, offset=1000)
+
+
+@gpu
+def test_position_outside_the_tables_gives_nan():
+    q, k = torch.randn(3, 1, 1, 8, device="cuda"), torch.randn(3, 1, 1, 8, device="cuda")
+    y, _ = fused_qk_norm_rope(q, k, None, None, *rotary_tables(4, 4, device="cuda"), positions=torch.tensor([0, 4, -1], device="cuda"))
+    assert torch.isnan(y[1:, ..., :4]).all() and torch.equal(y[1:, ..., 4:], q[1:, ..., 4:]) and not torch.isnan(y[0]).any()
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(0, 2, 2, 2, 64), (3, 0, 2, 2, 64), (3, 2, 0, 2, 64)])
+def test_empty(shape):
+    s, b, np_, ng, hn = shape
+    q = torch.randn(s, b, np_, hn, device="cuda").requires_grad_()
+    k = torch.randn(s, b, ng, hn, device="cuda").requires_grad_()
+    w = torch.ones(hn, device="cuda").requires_grad_()
+    yq, yk = fused_qk_norm_rope(q, k, w, w, *rotary_tables(4, hn, device="cuda"))
+    grads = torch.autograd.grad((yq, yk), (q, k, w), (torch.ones_like(yq), torch.ones_like(yk)))
+    assert yq.shape == q.shape and grads[1].shape == k.shape and torch.isfinite(grads[2]).all()
+
+
+@gpu
+def test_zero_head_and_refusals():
+    z = torch.zeros(2, 1, 2, 64, device="cuda", dtype=torch.float16)
+    w = torch.ones(64, device="cuda")
+    y, _ = fused_qk_norm_rope(z, z, w, w)
+    assert (y == 0).all()
+    for bad in (z.double(), torch.zeros(2, 1, 2, 63, device="cuda"), torch.zeros(2, 1, 2, 514, device="cuda")):
+        with pytest.raises((ValueError, RuntimeError)):
+            fused_qk_norm_rope(bad, bad, torch.ones(bad.size(3), device="cuda"), torch.ones(bad.size(3), device="cuda"))
+
+
+@gpu
+def test_one_output_used_and_same_bits_again():
+    q = torch.randn(300, 3, 4, 64, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    k = torch.randn(300, 3, 2, 64, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    w = [torch.randn(64, device="cuda").requires_grad_() for _ in range(2)]
+    tabs = rotary_tables(300, 64, device="cuda")
+    yq, yk = fused_qk_norm_rope(q, k, *w, *tabs)
+    dy = torch.randn_like(yq)
+    a = torch.autograd.grad(yq, (q, k, *w), dy, retain_graph=True)
+    b = torch.autograd.grad(yq, (q, k, *w), dy, retain_graph=True)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    assert (a[1] == 0).all() and (a[3] == 0).all()
+    (g,) = torch.autograd.grad(yq.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@gpu
+def test_captured_and_replayed():
+    q = torch.randn(200, 2, 4, 128, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    k = torch.randn(200, 2, 2, 128, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    w = [torch.randn(128, device="cuda").requires_grad_() for _ in range(2)]
+    tabs = rotary_tables(4096, 128, device="cuda")
+    pos = torch.arange(200, device="cuda")
+    dy = torch.randn_like(q), torch.randn_like(k)
+
+    def step():
+        ys = fused_qk_norm_rope(q, k, *w, *tabs, positions=pos)
+        return (*ys, *torch.autograd.grad(ys, (q, k, *w), dy))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for n in range(3):
+        with torch.no_grad():
+            q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(n)))
+            pos.copy_(torch.randperm(4096, generator=torch.Generator().manual_seed(n))[:200])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step()):
+            assert torch.equal(a, b)
