@@ -25,13 +25,17 @@ struct GaArgs {
   uint64_t seed = 0;
   const int64_t* seed_dev = nullptr;  // step seed of a captured step (utils/graph_rng.py)
   float* lse = nullptr;               // [b, np, sq] log2-sum-exp2 of the base-2 scaled scores, +inf: no key seen
-  float* delta = nullptr;             // [b, np, sq] rowsum(dout * o)
-  uint32_t* rowh = nullptr;           // [b, np, sq] dropout row hashes (backward with dropout)
+  void* olo = nullptr;                // what rounding left of o, laid out like o (null: no backward follows)
+  // backward scratch, written by the dQ kernel for the dK / dV kernel
+  float* delta = nullptr;    // [b, np, sq] rowsum(dout * o)
+  uint32_t* rowh = nullptr;  // [b, np, sq] dropout row hashes (with dropout)
 };
 
 // partial results of the split-key forward, in floats (0: the forward needs none)
 int64_t ga_forward_workspace(const GaArgs& a);
 void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st);
-void ga_backward(int dt, const GaArgs& a, hipStream_t st);
+// partial sums of dK / dV, in floats (0: none)
+int64_t ga_backward_workspace(const GaArgs& a);
+void ga_backward(int dt, const GaArgs& a, float* ws, hipStream_t st);  // dk.p null: dQ only
 
 }  // namespace bh

@@ -25,6 +25,11 @@ using namespace m32;
 constexpr int kThreads = 256;  // 4 waves
 constexpr int kTileQ = 128;    // rows of a workgroup: 32 per wave
 constexpr int kBlk = 64;       // rows of the streamed operand per step
+#ifndef BH_GA_T1
+#define BH_GA_T1 2048
+#define BH_GA_T2 1024
+#define BH_GA_T3 512
+#endif
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- LDS images ------------------------------------------------------------------------------------------
@@ -87,8 +92,16 @@ template <typename T> BH_DEVICE i4v load_frag(const T* base, int64_t st, int row
   return i4v{0, 0, 0, 0};
 }
 
-template <typename T> BH_DEVICE T* at(const GaView& v, int b, int h) {
-  return reinterpret_cast<T*>(v.p) + (int64_t)b * v.sb + (int64_t)h * v.sh;
+template <typename T> BH_DEVICE T* at(const GaView& v, int b, int h, void* base) {
+  return reinterpret_cast<T*>(base) + (int64_t)b * v.sb + (int64_t)h * v.sh;
+}
+template <typename T> BH_DEVICE T* at(const GaView& v, int b, int h) { return at<T>(v, b, h, v.p); }
+// 4 output values and, for the backward pass, what their rounding left over
+template <typename T> BH_DEVICE void store_out(T* out, T* rest, float a, float b, float c, float d) {
+  store4<T>(out, a, b, c, d);
+  if (rest)
+    store4<T>(rest, a - to_f<T>(from_f<T>(a)), b - to_f<T>(from_f<T>(b)), c - to_f<T>(from_f<T>(c)),
+              d - to_f<T>(from_f<T>(d)));
 }
 BH_DEVICE uint64_t eff_seed(const GaArgs& a) {
   return a.seed_dev ? a.seed ^ ((uint64_t)*a.seed_dev * 0x9E3779B97F4A7C15ull) : a.seed;
@@ -258,14 +271,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
   l = half_sum(l);
   if (myq < a.sq) {
     const float inv = l > 0.f ? (DROP ? kscale : 1.f) / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
-    T* out = at<T>(a.o, b, head) + (int64_t)myq * a.o.st;
+    const int64_t at_o = (int64_t)myq * a.o.st + 4 * h;
+    T* out = at<T>(a.o, b, head) + at_o;
+    T* rest = a.olo ? at<T>(a.o, b, head, a.olo) + at_o : nullptr;
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (32 * dn + 8 * q < a.hn)
-          store4<T>(out + 32 * dn + 8 * q + 4 * h, O[dn][4 * q] * inv, O[dn][4 * q + 1] * inv, O[dn][4 * q + 2] * inv,
-                    O[dn][4 * q + 3] * inv);
+          store_out<T>(out + 32 * dn + 8 * q, rest ? rest + 32 * dn + 8 * q : nullptr, O[dn][4 * q] * inv,
+                       O[dn][4 * q + 1] * inv, O[dn][4 * q + 2] * inv, O[dn][4 * q + 3] * inv);
     if (h == 0) a.lse[(int64_t)bh * a.sq + myq] = l == 0.f ? INFINITY : m + __log2f(l);
   }
 }
@@ -400,10 +415,14 @@ __global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, 
   }
   const int jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
   const float inv = lw > 0.f ? 1.f / lw : (lw == 0.f ? 0.f : lw);
-  T* out = at<T>(a.o, b, head) + (int64_t)iq * a.o.st;
+  const int64_t at_o = (int64_t)iq * a.o.st + d0;
+  T* out = at<T>(a.o, b, head) + at_o;
+  T* rest = a.olo ? at<T>(a.o, b, head, a.olo) + at_o : nullptr;
 #pragma unroll
   for (int d = 0; d < PER; d += 4)
-    if (d0 + d < a.hn) store4<T>(out + d0 + d, acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv, acc[d + 3] * inv);
+    if (d0 + d < a.hn)
+      store_out<T>(out + d, rest ? rest + d : nullptr, acc[d] * inv, acc[d + 1] * inv, acc[d + 2] * inv,
+                   acc[d + 3] * inv);
   if (d0 == 0) a.lse[((int64_t)b * a.np + head) * a.sq + iq] = lw == 0.f ? INFINITY : mm + __log2f(lw);
 }
 
@@ -434,37 +453,29 @@ __global__ __launch_bounds__(kThreads) void k_ga_join(GaArgs a, int rtiles, int 
   }
   const int b = unit / a.ng, g = unit % a.ng, jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (d < a.hn)
-    store4<T>(at<T>(a.o, b, head) + (int64_t)iq * a.o.st + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  if (d < a.hn) {
+    const int64_t at_o = (int64_t)iq * a.o.st + d;
+    store_out<T>(at<T>(a.o, b, head) + at_o, a.olo ? at<T>(a.o, b, head, a.olo) + at_o : nullptr, acc[0] * inv,
+                 acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  }
   if (d == 0) a.lse[((int64_t)b * a.np + head) * a.sq + iq] = l == 0.f ? INFINITY : mm + __log2f(l);
 }
 
 // ---- backward --------------------------------------------------------------------------------------------
-// delta = rowsum(dO * O), 16 lanes a row of up to 128 values; with dropout also the row hashes
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_ga_delta(GaArgs a) {
-  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 16;  // (b * np + head) * sq + q
-  const int sub = threadIdx.x & 15;
-  if (row >= (int64_t)a.b * a.np * a.sq) return;
-  const int bh = (int)(row / a.sq), q = (int)(row - (int64_t)bh * a.sq), b = bh / a.np, head = bh % a.np;
-  float acc = 0.f;
-  if (8 * sub < a.hn) {
-    float o[8], d[8];
-    VecIO<T>::load(at<const T>(a.o, b, head) + (int64_t)q * a.o.st + 8 * sub, o);
-    VecIO<T>::load(at<const T>(a.dout, b, head) + (int64_t)q * a.dout.st + 8 * sub, d);
+// sum of the products of 8 values of two operand fragments
+template <typename T> BH_DEVICE float dot8(i4v x, i4v y, float acc) {
+  typedef T t8v __attribute__((ext_vector_type(8)));
+  const t8v a = __builtin_bit_cast(t8v, x), b = __builtin_bit_cast(t8v, y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = fmaf(o[i], d[i], acc);
-  }
-#pragma unroll
-  for (int s = 1; s < 16; s <<= 1) acc += __shfl_xor(acc, s);
-  if (sub == 0) {
-    a.delta[row] = acc;
-    if (a.rowh) a.rowh[row] = row_hash(eff_seed(a), bh, q);
-  }
+  for (int i = 0; i < 8; ++i) acc = fmaf(to_f<T>(a[i]), to_f<T>(b[i]), acc);
+  return acc;
 }
 
 // dQ: the forward's layout. S^T = K Q^T and dP^T = V dO^T from row fragments, dS^T stays in registers and feeds
-// dQ^T = K^T dS^T (K^T by transposed reads of the same image).
+// dQ^T = K^T dS^T (K^T by transposed reads of the same image). It runs before the dK / dV kernel and leaves
+// delta (and the dropout row hashes) for it: its dO fragments are in registers anyway. delta is taken from O
+// with its rounding's rest: where few keys carry a query, dP - delta cancels and the rounding of O alone would
+// be a good part of dS (GPT-2-medium's shape: error of dQ 2.5e-3 instead of 2.35e-3, dS rounding included).
 template <typename T, int D, bool DROP>
 __global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_t thresh, float kscale) {
   constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
@@ -488,8 +499,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_
   }
   const float c = a.scale * kLog2e;
   const int64_t row = (int64_t)bh * a.sq + min(myq, a.sq - 1);
-  const float nl = -a.lse[row], dl = a.delta[row];
-  const uint32_t rowh = DROP ? a.rowh[row] : 0u;
+  const float nl = -a.lse[row];
+  float dl = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    dl = dot8<T>(load_frag<T>(at<const T>(a.o, b, head), a.o.st, myq, a.sq, 16 * s + 8 * h, a.hn), df[s], dl);
+    dl = dot8<T>(load_frag<T>(at<const T>(a.o, b, head, a.olo), a.o.st, myq, a.sq, 16 * s + 8 * h, a.hn), df[s], dl);
+  }
+  dl = half_sum(dl);
+  const uint32_t rowh = DROP ? row_hash(eff_seed(a), bh, myq) : 0u;
+  if (h == 0 && myq < a.sq) {
+    a.delta[row] = dl;
+    if (DROP) a.rowh[row] = rowh;
+  }
   f16v acc[DN];
 #pragma unroll
   for (int dn = 0; dn < DN; ++dn) acc[dn] = zero16();
@@ -560,26 +582,37 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_
   }
 }
 
-// dK / dV: workgroup = 4 waves x 32 keys of one key head, the key on the lane; it walks the 64-query blocks of
-// all r query heads of the group, so the gradients of shared heads are summed in the accumulators (no atomics,
-// one order). S = Q K^T and dP = dO V^T from row fragments (K / V stay in registers), P and dS feed
-// dV^T = dO^T P and dK^T = Q^T dS from the accumulators. -L, delta and the row hashes of the block ride along.
+// dK / dV: workgroup = 4 waves x 32 keys of one key head, the key on the lane; it walks the query blocks of all
+// r query heads of the group, so the gradients of shared heads are summed in the accumulators (no atomics, one
+// order). S = Q K^T and dP = dO V^T from row fragments, P and dS feed dV^T = dO^T P and dK^T = Q^T dS from the
+// accumulators. L, delta and the row hashes of a block ride along.
+// Registers decide the shape: at D = 128 the accumulators take 128 of the 256 that two waves a SIMD leave, so V
+// is read from LDS again each block (K stays in registers) and blocks are 32 queries; at D = 64 both stay in
+// registers and blocks are 64.
+// The blocks of a key tile are cut into `splits` runs (few key tiles, or a causal mask that gives the first
+// tiles most of the work); their fp32 sums then meet in k_ga_dkdv_join, in order.
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, uint32_t thresh, float kscale) {
-  constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32, BUF = 2 * IMG + 3 * 256;
-  __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+__global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int splits, uint32_t thresh, float kscale,
+                                                         float* __restrict__ ws) {
+  constexpr int RB = 2 * D, QB = D == 64 ? 64 : 32, IMG = QB * RB, KS = D / 16, DN = D / 32, BUF = 2 * IMG + 3 * 256;
+  constexpr bool VLDS = D == 128;
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF + (VLDS ? kTileQ * RB : 0)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const int r = a.np / a.ng;
-  const Problem pr = problem(nx, a.b * a.ng, 1, a.causal);
+  const Problem pr = problem(nx, a.b * a.ng, splits, a.causal);
   const int b = pr.unit / a.ng, g = pr.unit % a.ng;
   const int nk = seq_keys(a, b), off = a.sk - a.sq;
   const int k0 = pr.tile * kTileQ, k0w = k0 + wave * 32, mykey = k0w + r32;
-  i4v kf[KS], vf[KS];
+  const Frag<D> fr(lane);
+  char* const vtile = smem + 2 * BUF + wave * 32 * RB;  // this wave's 32 keys
+  i4v kf[KS], vf[VLDS ? 1 : KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     kf[s] = load_frag<T>(at<const T>(a.k, b, g), a.k.st, mykey, nk, 16 * s + 8 * h, a.hn);
-    vf[s] = load_frag<T>(at<const T>(a.v, b, g), a.v.st, mykey, nk, 16 * s + 8 * h, a.hn);
+    const i4v v = load_frag<T>(at<const T>(a.v, b, g), a.v.st, mykey, nk, 16 * s + 8 * h, a.hn);
+    if (VLDS) *reinterpret_cast<i4v*>(vtile + (fr.r0 ^ (s << 5))) = v;
+    else vf[VLDS ? 0 : s] = v;
   }
   const float c = a.scale * kLog2e;
   f16v dK[DN], dV[DN];
@@ -588,47 +621,53 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, uint3
   // queries that see a key of the tile: key - off <= i < key - off + window
   int qbeg = 0, qend = k0 < nk ? a.sq : 0;
   if (a.causal) {
-    qbeg = max(0, k0 - off) & ~(kBlk - 1);
+    qbeg = max(0, k0 - off) & ~(QB - 1);
     qend = min(qend, min(k0 + kTileQ, nk) - 1 - off + a.window);
   }
-  const int nqb = qend > qbeg ? (qend - qbeg + kBlk - 1) / kBlk : 0, total = nqb * r;
-  const Stage<D, kBlk, 4> sq(a.q.st, a.hn, wave, lane), sd(a.dout.st, a.hn, wave, lane);
-  const Frag<D> fr(lane);
-  auto stage = [&](int it, char* buf) {
-    const int j = it / nqb, q0 = qbeg + (it - j * nqb) * kBlk, head = g * r + j;
+  const int nqb = qend > qbeg ? (qend - qbeg + QB - 1) / QB : 0, total = nqb * r;
+  const int it0 = (int)((int64_t)total * pr.j / splits), it1 = (int)((int64_t)total * (pr.j + 1) / splits);
+  const Stage<D, QB, 4> sq(a.q.st, a.hn, wave, lane), sd(a.dout.st, a.hn, wave, lane);
+  auto stage = [&](int j, int q0, char* buf) {
+    const int head = g * r + j;
     sq.issue(at<const T>(a.q, b, head) + (int64_t)q0 * a.q.st, a.q.st, a.hn, a.sq - q0, buf, wave);
     sd.issue(at<const T>(a.dout, b, head) + (int64_t)q0 * a.dout.st, a.dout.st, a.hn, a.sq - q0, buf + IMG, wave);
     // rows past the last query read as zeros: their Q and dO rows are zero too, so P = 1 meets dO = 0
     const int64_t row = ((int64_t)b * a.np + head) * a.sq + q0;
-    const uint32_t bytes = 4u * (uint32_t)min(a.sq - q0, kBlk);
+    const uint32_t bytes = 4u * (uint32_t)min(a.sq - q0, QB);
     const unsigned l = __builtin_amdgcn_readfirstlane(lds_addr(buf + 2 * IMG));
     if (wave == 0) dma4(make_rsrc(a.lse + row, bytes), lane * 4, l);
     else if (wave == 1) dma4(make_rsrc(a.delta + row, bytes), lane * 4, l + 256);
     else if (DROP && wave == 2) dma4(make_rsrc(a.rowh + row, bytes), lane * 4, l + 512);
   };
-  if (total > 0) stage(0, smem);
-  for (int it = 0; it < total; ++it) {
-    const int j = it / nqb, q0 = qbeg + (it - j * nqb) * kBlk;
-    const char* qimg = smem + (it & 1) * BUF;
+  int j = nqb ? it0 / nqb : 0, q0 = qbeg + (it0 - j * nqb) * QB;  // head of the group and first query of a block
+  if (it0 < it1) stage(j, q0, smem);
+  for (int it = it0; it < it1; ++it) {
+    const int qb = q0;
+    const char* qimg = smem + ((it - it0) & 1) * BUF;
     const char* dimg = qimg + IMG;
     const float* lp = reinterpret_cast<const float*>(dimg + IMG);
     wait_vmcnt<0>();
     lds_barrier();
-    if (it + 1 < total) stage(it + 1, smem + ((it + 1) & 1) * BUF);
+    q0 += QB;
+    if (q0 >= qend) {
+      q0 = qbeg;
+      ++j;
+    }
+    if (it + 1 < it1) stage(j, q0, smem + ((it - it0 + 1) & 1) * BUF);
     if (k0w >= nk) continue;
-    if (a.causal && (q0 + kBlk - 1 + off < k0w || q0 + off - a.window + 1 > k0w + 31)) continue;
-    const bool ml = a.causal && q0 + off < k0w + 31;                             // some query precedes some key
-    const bool mh = a.causal && q0 + kBlk - 1 + off - a.window + 1 > k0w;        // some key left the window
+    if (a.causal && (qb + QB - 1 + off < k0w || qb + off - a.window + 1 > k0w + 31)) continue;
+    const bool ml = a.causal && qb + off < k0w + 31;                       // some query precedes some key
+    const bool mh = a.causal && qb + QB - 1 + off - a.window + 1 > k0w;    // some key left the window
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < QB / 32; ++t) {
       f16v S = zero16(), P = zero16();
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         S = Mfma<T>::run(fr.row(qimg, 32 * t, s), kf[s], S);
-        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), vf[s], P);  // dP
+        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), VLDS ? fr.row(vtile, 0, s) : vf[VLDS ? 0 : s], P);  // dP
       }
-      if (ml) mask_lo(S, mykey - off - q0 - 4 * h - 32 * t);
-      if (mh) mask_hi(S, mykey - off + a.window - 1 - q0 - 4 * h - 32 * t);
+      if (ml) mask_lo(S, mykey - off - qb - 4 * h - 32 * t);
+      if (mh) mask_hi(S, mykey - off + a.window - 1 - qb - 4 * h - 32 * t);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float* at4 = lp + 32 * t + 8 * q + 4 * h;
@@ -661,25 +700,60 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, uint3
       }
     }
   }
-  if (mykey < a.sk) {  // keys past the sequence's length take zeros, whatever their lanes held
-    const bool real = mykey < nk;
-    T* dk = at<T>(a.dk, b, g) + (int64_t)mykey * a.dk.st;
-    T* dv = at<T>(a.dv, b, g) + (int64_t)mykey * a.dv.st;
+  if (mykey >= a.sk) return;
+  const bool real = mykey < nk;  // keys past the sequence's length take zeros, whatever their lanes held
+  if (splits > 1) {
+    float* w = ws + (((int64_t)pr.j * a.b * a.ng + pr.unit) * a.sk + mykey) * (2 * D) + 4 * h;
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (32 * dn + 8 * q < a.hn) {
-          float x[4], y[4];
+      for (int q = 0; q < 4; ++q) {
+        f4v x, y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = real ? dK[dn][4 * q + e] * a.scale : 0.f;
-            y[e] = real ? dV[dn][4 * q + e] : 0.f;
-          }
-          store4<T>(dk + 32 * dn + 8 * q + 4 * h, x[0], x[1], x[2], x[3]);
-          store4<T>(dv + 32 * dn + 8 * q + 4 * h, y[0], y[1], y[2], y[3]);
+        for (int e = 0; e < 4; ++e) {
+          x[e] = real ? dK[dn][4 * q + e] * a.scale : 0.f;
+          y[e] = real ? dV[dn][4 * q + e] : 0.f;
         }
+        *reinterpret_cast<f4v*>(w + 32 * dn + 8 * q) = x;
+        *reinterpret_cast<f4v*>(w + D + 32 * dn + 8 * q) = y;
+      }
+    return;
   }
+  T* dk = at<T>(a.dk, b, g) + (int64_t)mykey * a.dk.st + 4 * h;
+  T* dv = at<T>(a.dv, b, g) + (int64_t)mykey * a.dv.st + 4 * h;
+#pragma unroll
+  for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (32 * dn + 8 * q < a.hn) {
+        float x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = real ? dK[dn][4 * q + e] * a.scale : 0.f;
+          y[e] = real ? dV[dn][4 * q + e] : 0.f;
+        }
+        store4<T>(dk + 32 * dn + 8 * q, x[0], x[1], x[2], x[3]);
+        store4<T>(dv + 32 * dn + 8 * q, y[0], y[1], y[2], y[3]);
+      }
+}
+
+// dK / dV = sums of the splits' fp32 rows, in order; 2 D / 4 threads a key, 4 values each
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void k_ga_dkdv_join(GaArgs a, int splits, const float* __restrict__ ws) {
+  constexpr int TPR = 2 * D / 4;
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = id / TPR, rows = (int64_t)a.b * a.ng * a.sk;
+  if (row >= rows) return;
+  const int x = (int)(id % TPR) * 4, d = x % D;
+  if (d >= a.hn) return;
+  f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const f4v v = *reinterpret_cast<const f4v*>(ws + ((int64_t)s * rows + row) * (2 * D) + x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += v[i];
+  }
+  const int unit = (int)(row / a.sk), key = (int)(row - (int64_t)unit * a.sk);
+  const GaView& o = x < D ? a.dk : a.dv;
+  store4<T>(at<T>(o, unit / a.ng, unit % a.ng) + (int64_t)key * o.st + d, acc[0], acc[1], acc[2], acc[3]);
 }
 
 inline void check_launch(const char* what) {
@@ -712,14 +786,23 @@ struct SplitPlan {
 SplitPlan split_plan(const GaArgs& a) {
   SplitPlan p;
   const int64_t tiled = (int64_t)((a.sq + kTileQ - 1) / kTileQ) * a.b * a.np;
-  if (a.p_drop > 0.f || tiled >= 256) return p;
   const int64_t rows = (int64_t)(a.np / a.ng) * a.sq, rt = (rows + 31) / 32, probs = rt * a.b * a.ng;
-  const int64_t want = std::max<int64_t>(1, 256 / probs), most = std::max(1, (a.sk + 127) / 128);
+  if (a.p_drop > 0.f || (tiled >= 256 && rows > 64)) return p;
+  const int64_t want = std::max<int64_t>(1, BH_GA_T3 / probs), most = std::max(1, (a.sk + 127) / 128);
   const int64_t s = std::min(want, most);
   p.rtiles = (int)rt;
   p.chunk = (int)((((int64_t)a.sk + s - 1) / s + 127) / 128 * 128);
   p.splits = (int)(((int64_t)a.sk + p.chunk - 1) / p.chunk);
   return p;
+}
+
+// runs of a key tile's query blocks: enough workgroups for four rounds of the card's 512 places, at least 4
+// blocks of 64 queries each
+int dkdv_splits(const GaArgs& a) {
+  const int64_t wgs = (int64_t)((a.sk + kTileQ - 1) / kTileQ) * a.b * a.ng;
+  const int64_t blocks = ((int64_t)std::min<int64_t>(a.sq, (int64_t)a.window + kTileQ) + 63) / 64 * (a.np / a.ng);
+  const int64_t target = a.causal ? BH_GA_T1 : BH_GA_T2;
+  return (int)std::max<int64_t>(1, std::min(target / wgs, blocks / 4));
 }
 
 }  // namespace
@@ -757,21 +840,27 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
   check_launch("ga_forward");
 }
 
-void ga_backward(int dt, const GaArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.b * a.np * a.sq;
-  const dim3 gd((unsigned)((rows * 16 + kThreads - 1) / kThreads));
-  const int nq = (a.sq + kTileQ - 1) / kTileQ, nkt = (a.sk + kTileQ - 1) / kTileQ;
+int64_t ga_backward_workspace(const GaArgs& a) {
+  const int n = dkdv_splits(a);
+  return n > 1 ? (int64_t)n * a.b * a.ng * a.sk * 2 * (a.hn <= 64 ? 64 : 128) : 0;
+}
+
+void ga_backward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
+  const int nq = (a.sq + kTileQ - 1) / kTileQ, nkt = (a.sk + kTileQ - 1) / kTileQ, splits = dkdv_splits(a);
   dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
     using T = typename decltype(t)::type;
     constexpr int D = decltype(dd)::value;
     constexpr bool DROP = decltype(drop)::value;
-    hipLaunchKernelGGL((k_ga_delta<T>), gd, dim3(kThreads), 0, st, a);
-    if (a.dk.p)
-      hipLaunchKernelGGL((k_ga_dkdv<T, D, DROP>), dim3((unsigned)((int64_t)nkt * a.b * a.ng)), dim3(kThreads), 0, st, a,
-                         nkt, keep_thresh(a), keep_scale(a));
-    if (a.dq.p)
-      hipLaunchKernelGGL((k_ga_dq<T, D, DROP>), dim3((unsigned)((int64_t)nq * a.b * a.np)), dim3(kThreads), 0, st, a,
-                         nq, keep_thresh(a), keep_scale(a));
+    hipLaunchKernelGGL((k_ga_dq<T, D, DROP>), dim3((unsigned)((int64_t)nq * a.b * a.np)), dim3(kThreads), 0, st, a, nq,
+                       keep_thresh(a), keep_scale(a));
+    if (!a.dk.p) return;
+    hipLaunchKernelGGL((k_ga_dkdv<T, D, DROP>), dim3((unsigned)((int64_t)nkt * a.b * a.ng * splits)), dim3(kThreads), 0,
+                       st, a, nkt, splits, keep_thresh(a), keep_scale(a), ws);
+    if (splits > 1) {
+      const int64_t n = (int64_t)a.b * a.ng * a.sk * (2 * D / 4);
+      hipLaunchKernelGGL((k_ga_dkdv_join<T, D>), dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st,
+                         a, splits, ws);
+    }
   });
   check_launch("ga_backward");
 }

@@ -10,7 +10,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..._autocast_utils import _cast_if_autocast_enabled
 from ..._native import submodule
@@ -75,34 +74,17 @@ def _attention_torch(q, k, v, lens, causal, window, scale, p, seed):
     return torch.matmul(prob, vf).permute(2, 0, 1, 3).to(q.dtype).contiguous()
 
 
-class GroupedAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lens, causal, window, scale, p, seed, seed_dev):
-        out, lse = submodule("grouped_attention").forward(q, k, v, causal, window, lens, scale, p, seed, seed_dev)
-        ctx.save_for_backward(q, k, v, out, lse, lens)
-        ctx.args = (causal, window, scale, p, seed)
-        # the step seed a captured step advances in place: read again by the backward of the same step
-        ctx.seed_dev = seed_dev
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, lens = ctx.saved_tensors
-        causal, window, scale, p, seed = ctx.args
-        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq, dk, dv = submodule("grouped_attention").backward(
-            _usable(dout), q, k, v, out, lse, causal, window, lens, scale, p, seed, ctx.seed_dev, need_q, need_kv)
-        return dq, dk, dv, None, None, None, None, None, None, None
-
-
-def _usable(t: torch.Tensor) -> torch.Tensor:
-    """``t``, copied when the kernels cannot address it (head_dim not contiguous, strides or base off 16 bytes,
-    positions overlapping or 2^24 elements and more apart)."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and (
-        t.size(0) <= 1 or t.size(3) <= t.stride(0) < 1 << 24) and all(
-        t.stride(d) % 8 == 0 for d in range(3) if t.size(d) > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _check(query, key, value):
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.dim() != 4:
+            raise ValueError(f"fused_grouped_attention: {name} must be [s, b, heads, head_dim], got {tuple(t.shape)}")
+    if key.shape != value.shape or key.size(1) != query.size(1) or key.size(3) != query.size(3):
+        raise ValueError(f"fused_grouped_attention: query {tuple(query.shape)}, key {tuple(key.shape)} and value "
+                         f"{tuple(value.shape)} do not fit")
+    if key.size(2) < 1 or query.size(2) < 1 or query.size(2) % key.size(2):
+        raise ValueError(f"fused_grouped_attention: {query.size(2)} query heads are no multiple of {key.size(2)} key heads")
+    if not query.dtype == key.dtype == value.dtype:
+        raise ValueError("fused_grouped_attention: query, key and value must have one dtype")
 
 
 def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, causal: bool = False,
@@ -130,19 +112,11 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
             through ``utils.graph_rng``).
 
     A query that sees no key gives zeros and takes no gradient. Returns [sq, b, np, hn], contiguous."""
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.dim() != 4:
-            raise ValueError(f"fused_grouped_attention: {name} must be [s, b, heads, head_dim], got {tuple(t.shape)}")
-    if key.shape != value.shape or key.size(1) != query.size(1) or key.size(3) != query.size(3):
-        raise ValueError(f"fused_grouped_attention: query {tuple(query.shape)}, key {tuple(key.shape)} and value "
-                         f"{tuple(value.shape)} do not fit")
-    if key.size(2) < 1 or query.size(2) < 1 or query.size(2) % key.size(2):
-        raise ValueError(f"fused_grouped_attention: {query.size(2)} query heads are no multiple of {key.size(2)} key heads")
     if window is not None and (not causal or int(window) < 1):
         raise ValueError("fused_grouped_attention: window needs causal=True and must be at least 1")
     if not 0.0 <= dropout_p < 1.0:
         raise ValueError(f"fused_grouped_attention: dropout_p must be in [0, 1), got {dropout_p}")
-    scale = float(scale) if scale is not None else query.size(3) ** -0.5
+    scale = float(scale) if scale is not None else query.size(-1) ** -0.5
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"fused_grouped_attention: scale must be positive, got {scale}")
     if key_lengths is not None:
@@ -151,8 +125,6 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
         if key_lengths.device != query.device:
             raise ValueError("fused_grouped_attention: key_lengths must be on the query's device")
     query, key, value = _cast_if_autocast_enabled(query, key, value)
-    if not query.dtype == key.dtype == value.dtype:
-        raise ValueError("fused_grouped_attention: query, key and value must have one dtype")
     p = float(dropout_p) if training else 0.0
     seed_dev = None
     if p > 0 and seed is None:
@@ -160,17 +132,14 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
 
         seed, seed_dev = _seed_pair()
     seed = _signed64(int(seed)) if p > 0 else 0
-    if not query.is_cuda:
-        lens = None if key_lengths is None else key_lengths.clamp(0, key.size(0))
-        with torch.autocast("cpu", enabled=False):
-            return _attention_torch(query, key, value, lens, causal, int(window or 0), scale, p, seed)
-    lens = None
-    if key_lengths is not None:
-        lens = key_lengths.clamp(0, key.size(0)) if key_lengths.dtype != torch.int32 else key_lengths
-        lens = lens.to(torch.int32).contiguous()
-    args = (_usable(query), _usable(key), _usable(value), lens, bool(causal), int(window or 0), scale, p, seed, seed_dev)
-    with torch.autocast("cuda", enabled=False):
-        if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
-            return GroupedAttentionFn.apply(*args)
-        q, k, v, lens, causal, window, scale, p, seed, seed_dev = args
-        return submodule("grouped_attention").forward(q, k, v, causal, window, lens, scale, p, seed, seed_dev)[0]
+    window = 0 if window is None else int(window)
+    if query.is_cuda:  # the native call checks the operands
+        if key_lengths is not None:
+            if key_lengths.dtype != torch.int32:
+                key_lengths = key_lengths.clamp(0, key.size(0)).to(torch.int32)
+            key_lengths = key_lengths.contiguous()
+        return submodule("grouped_attention").attention(query, key, value, key_lengths, causal, window, scale, p, seed,
+                                                        seed_dev)
+    _check(query, key, value)
+    lens = None if key_lengths is None else key_lengths.clamp(0, key.size(0))
+    return _attention_torch(query, key, value, lens, causal, window, scale, p, seed)

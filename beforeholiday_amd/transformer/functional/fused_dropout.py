@@ -36,21 +36,19 @@ def dropout_keep(seed: int, n: int, p: float, device=None) -> torch.Tensor:
 
 
 class CounterDropoutFn(torch.autograd.Function):
-    """x -> keep ? x / (1 - p) : 0; its backward is itself on the gradient (any number of times)."""
+    """x -> keep ? x / (1 - p) : 0 on the CPU; its backward is itself on the gradient (any number of times)."""
 
     @staticmethod
-    def forward(ctx, x, p, seed, seed_dev):
-        ctx.args = (p, seed, seed_dev)
+    def forward(ctx, x, p, seed):
+        ctx.args = (p, seed)
         scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
-        if x.is_cuda:
-            return submodule("counter_dropout").apply(x.contiguous(), _threshold(p), scale, seed, seed_dev)
         keep = dropout_keep(seed, x.numel(), p, x.device).view(x.shape)
         y = x.to(torch.promote_types(x.dtype, torch.float32)) * scale
         return torch.where(keep, y, torch.zeros((), dtype=y.dtype)).to(x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
-        return CounterDropoutFn.apply(dy, *ctx.args), None, None, None
+        return CounterDropoutFn.apply(dy, *ctx.args), None, None
 
 
 def fused_dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, *, seed: Optional[int] = None,
@@ -84,4 +82,7 @@ def fused_dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, *, see
             seed, seed_dev = graph_rng.next_salt(stream), graph_rng.step_seed()
         else:
             seed = dropout_seed(model_parallel)
-    return CounterDropoutFn.apply(x, float(p), _signed64(int(seed)), seed_dev)
+    p, seed = float(p), _signed64(int(seed))
+    if x.is_cuda:
+        return submodule("counter_dropout").dropout(x, _threshold(p), 1.0 / (1.0 - p) if p < 1.0 else 0.0, seed, seed_dev)
+    return CounterDropoutFn.apply(x, p, seed)

@@ -9,7 +9,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..._native import submodule
 
@@ -54,47 +53,7 @@ def _qk_norm_rope_torch(q, k, wq, wk, cos, sin, positions, offset, eps, interlea
     return tuple(outs)
 
 
-class QKNormRopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, offset, eps, interleaved):
-        yq, yk = submodule("qk_norm_rope").forward(q, k, wq, wk, cos, sin, positions, offset, eps, interleaved)
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        ctx.args = (offset, eps, interleaved)
-        return yq, yk
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dyq, dyk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        dq, dk, dw = submodule("qk_norm_rope").backward(_usable(dyq), _usable(dyk), q, k, wq, wk, cos, sin, positions,
-                                                        *ctx.args)
-        dwq, dwk = (dw[0].to(wq.dtype), dw[1].to(wk.dtype)) if wq is not None else (None, None)
-        return dq, dk, dwq, dwk, None, None, None, None, None, None
-
-
-def _usable(t):
-    return t if t.stride(3) == 1 else t.clone(memory_format=torch.contiguous_format)
-
-
-def fused_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, query_weight: Optional[torch.Tensor] = None,
-                       key_weight: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
-                       sin: Optional[torch.Tensor] = None, *, positions: Optional[torch.Tensor] = None, offset: int = 0,
-                       eps: float = 1e-6, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
-    """RMS-normalises every head of ``query`` [s, b, np, hn] and ``key`` [s, b, ng, hn] over hn, scales it by
-    ``query_weight`` / ``key_weight`` [hn], then rotates its first ``2 * cos.size(1)`` values by the angle of its
-    position; the rest of the head passes through. Math in fp32, one rounding. Differentiable (once) in query, key and
-    the weights.
-
-    Args:
-        query, key: fp32 / fp16 / bf16, any strides (head_dim not contiguous: copied), hn even and at most 512.
-        query_weight, key_weight: both or none (no norm); fp32 / fp16 / bf16.
-        cos, sin: fp32 [positions, rot / 2] tables (:func:`rotary_tables`), both or none (no rotation). Not
-            differentiated.
-        positions: integer [s] or [s, b] rows of the tables; one outside them gives NaN in the rotated values.
-            Default: offset + 0 .. s - 1, which must fit the tables.
-        interleaved: pairs are neighbours (2 i, 2 i + 1); default: (i, i + rot / 2).
-
-    Returns the new query and key, contiguous."""
+def _check(query, key, query_weight, key_weight, cos, sin, positions, offset):
     for name, t in (("query", query), ("key", key)):
         if t.dim() != 4:
             raise ValueError(f"fused_qk_norm_rope: {name} must be [s, b, heads, head_dim], got {tuple(t.shape)}")
@@ -126,19 +85,30 @@ def fused_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, query_weight: Opt
         elif offset < 0 or offset + query.size(0) > cos.size(0):
             raise ValueError(f"fused_qk_norm_rope: positions {offset} .. {offset + query.size(0) - 1} do not fit tables of "
                              f"{cos.size(0)}")
-    else:
-        positions, offset = None, 0
-    if not query.is_cuda:
-        return _qk_norm_rope_torch(query, key, query_weight, key_weight, cos, sin, positions, int(offset), eps,
-                                   interleaved)
-    if cos is not None:
-        cos, sin = cos.detach().contiguous(), sin.detach().contiguous()
-    if query_weight is not None:
-        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
-    args = (_usable(query), _usable(key), query_weight, key_weight, cos, sin, positions, int(offset), float(eps),
-            bool(interleaved))
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or (
-            query_weight is not None and (query_weight.requires_grad or key_weight.requires_grad))):
-        return QKNormRopeFn.apply(*args)
-    yq, yk = submodule("qk_norm_rope").forward(*args)
-    return yq, yk
+
+
+def fused_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, query_weight: Optional[torch.Tensor] = None,
+                       key_weight: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                       sin: Optional[torch.Tensor] = None, *, positions: Optional[torch.Tensor] = None, offset: int = 0,
+                       eps: float = 1e-6, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS-normalises every head of ``query`` [s, b, np, hn] and ``key`` [s, b, ng, hn] over hn, scales it by
+    ``query_weight`` / ``key_weight`` [hn], then rotates its first ``2 * cos.size(1)`` values by the angle of its
+    position; the rest of the head passes through. Math in fp32, one rounding. Differentiable (once) in query, key and
+    the weights.
+
+    Args:
+        query, key: fp32 / fp16 / bf16, any strides (head_dim not contiguous: copied), hn even and at most 512.
+        query_weight, key_weight: both or none (no norm); fp32 / fp16 / bf16.
+        cos, sin: fp32 [positions, rot / 2] tables (:func:`rotary_tables`), both or none (no rotation). Not
+            differentiated.
+        positions: integer [s] or [s, b] rows of the tables; one outside them gives NaN in the rotated values.
+            Default: offset + 0 .. s - 1, which must fit the tables.
+        interleaved: pairs are neighbours (2 i, 2 i + 1); default: (i, i + rot / 2).
+
+    Returns the new query and key, contiguous."""
+    offset = int(offset)
+    if query.is_cuda:  # the native call checks the operands
+        return tuple(submodule("qk_norm_rope").norm_rope(query, key, query_weight, key_weight, cos, sin, positions, offset,
+                                                         eps, interleaved))
+    _check(query, key, query_weight, key_weight, cos, sin, positions, offset)
+    return _qk_norm_rope_torch(query, key, query_weight, key_weight, cos, sin, positions, offset, eps, interleaved)
