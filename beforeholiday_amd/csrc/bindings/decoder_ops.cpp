@@ -311,7 +311,7 @@ bh::QkRopeArgs rope_args(const at::Tensor& q, const at::Tensor& k, const c10::op
   }
   a.eps = (float)eps;
   a.interleaved = interleaved;
-  a.vec = vec && hn % 8 == 0 && a.rot % 8 == 0;
+  a.vec = vec && hn % 8 == 0 && (interleaved || a.rot % 8 == 0);
   return a;
 }
 

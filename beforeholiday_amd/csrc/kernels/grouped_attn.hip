@@ -25,11 +25,6 @@ using namespace m32;
 constexpr int kThreads = 256;  // 4 waves
 constexpr int kTileQ = 128;    // rows of a workgroup: 32 per wave
 constexpr int kBlk = 64;       // rows of the streamed operand per step
-#ifndef BH_GA_T1
-#define BH_GA_T1 2048
-#define BH_GA_T2 1024
-#define BH_GA_T3 512
-#endif
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- LDS images ------------------------------------------------------------------------------------------
@@ -288,15 +283,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
 // ---- forward, keys split over waves and workgroups ---------------------------------------------------------
 // For grids that would leave the card empty (few queries: single tokens against a long cache). The 32 lanes of
 // a tile are packed rows of one key head -- all r query heads of its group x sq queries -- so a group's K / V
-// are read once; every wave walks its own 32-key blocks with its own LDS buffers (no barrier in the loop), the
-// four waves join through LDS and the splits through an fp32 workspace.
+// are read once. Every wave walks its own 32-key blocks through an LDS buffer of its own (no barrier in the
+// loop); eight waves on a CU with one block in flight each keep the memory busy (one block computed while the
+// next is in flight, with half the waves, measured slower: BH_DECODE). The waves join through LDS, the splits
+// through an fp32 workspace.
+constexpr int kSplitWaves = 8, kSplitKeys = 32 * kSplitWaves;
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk,
-                                                          float* __restrict__ ws) {
-  constexpr int RB = 2 * D, IMG = 32 * RB, KS = D / 16, DN = D / 32, NP = IMG / 1024;
+__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk,
+                                                                  float* __restrict__ ws) {
+  constexpr int RB = 2 * D, IMG = 32 * RB, KS = D / 16, DN = D / 32, NP = IMG / 1024, NW = kSplitWaves;
   constexpr int OS = D + 4;  // floats of a joined row: 4 of padding keep the 32 rows off one bank
-  __shared__ __attribute__((aligned(16))) char smem[4 * 4 * IMG > 4 * 32 * OS * 4 ? 4 * 4 * IMG : 4 * 32 * OS * 4];
-  __shared__ float sml[2][4][32];
+  constexpr int BYTES = NW * 2 * IMG > NW * 32 * OS * 4 ? NW * 2 * IMG : NW * 32 * OS * 4;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  __shared__ float sml[2][NW][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const int r = a.np / a.ng, rows = r * a.sq;
@@ -305,45 +304,39 @@ __global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, 
   const int unit = prob % units, rt = prob / units;
   const int b = unit / a.ng, g = unit % a.ng;
   const int nk = seq_keys(a, b), off = a.sk - a.sq;
-  const int myr = rt * 32 + r32, jq = min(myr, rows - 1);
-  const int j = jq / a.sq, i_q = jq - j * a.sq, pos = i_q + off;
   const T* K = at<const T>(a.k, b, g);
   const T* V = at<const T>(a.v, b, g);
+  const int k1 = min(nk, split * chunk + chunk), first = split * chunk + wave * 32;
+  const char* kimg = smem + wave * 2 * IMG;
+  const char* vimg = kimg + IMG;
+  const Stage<D, 32, 1> sk(a.k.st, a.hn, 0, lane), sv(a.v.st, a.hn, 0, lane);
+  auto stage = [&](int kb) {
+    sk.issue(K + (int64_t)kb * a.k.st, a.k.st, a.hn, nk - kb, kimg, 0);
+    sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, vimg, 0);
+  };
+  if (first < k1) stage(first);
+  const int myr = rt * 32 + r32, jq = min(myr, rows - 1);
+  const int j = jq / a.sq, i_q = jq - j * a.sq, pos = i_q + off;
   const T* Q = at<const T>(a.q, b, g * r) + (int64_t)j * a.q.sh;
   i4v qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = load_frag<T>(Q, a.q.st, i_q, a.sq, 16 * s + 8 * h, a.hn);
   const float c = a.scale * kLog2e;
+  const Frag<D> fr(lane);
   float m = -INFINITY, l = 0.f;
   f16v O[DN];
 #pragma unroll
   for (int dn = 0; dn < DN; ++dn) O[dn] = zero16();
-
-  const int k0 = split * chunk, k1 = min(nk, k0 + chunk);
-  // keys that some row of the tile sees (rows are query-major inside a head: any query may be in the tile)
-  char* mine = smem + wave * 4 * IMG;
-  const Stage<D, 32, 1> sk(a.k.st, a.hn, 0, lane), sv(a.v.st, a.hn, 0, lane);
-  const Frag<D> fr(lane);
-  auto stage = [&](int kb, char* buf) {
-    sk.issue(K + (int64_t)kb * a.k.st, a.k.st, a.hn, nk - kb, buf, 0);
-    sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, 0);
-  };
-  const int first = k0 + wave * 32;
-  if (first < k1) stage(first, mine);
-  int cur = 0;
-  for (int kb = first; kb < k1; kb += 128, cur ^= 1) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave is done with the other buffer
-    if (kb + 128 < k1) {
-      stage(kb + 128, mine + (cur ^ 1) * 2 * IMG);
-      wait_vmcnt<2 * NP>();
-    } else {
-      wait_vmcnt<0>();
-    }
-    const char* kimg = mine + cur * 2 * IMG;
-    const char* vimg = kimg + IMG;
+  for (int kb = first; kb < k1; kb += kSplitKeys) {
+    wait_vmcnt<0>();
     f16v S = zero16();
 #pragma unroll
     for (int s = 0; s < KS; ++s) S = Mfma<T>::run(fr.row(kimg, 0, s), qf[s], S);
+    i4v vf[2 * DN];
+#pragma unroll
+    for (int x = 0; x < 2 * DN; ++x) vf[x] = fr.tr(vimg, 16 * (x / DN), x % DN);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // both images are in registers: the next block may land
+    if (kb + kSplitKeys < k1) stage(kb + kSplitKeys);
     mask_hi(S, (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h);
     if (a.causal) mask_lo(S, pos - a.window + 1 - kb - 4 * h);
     const float mx = half_max(tile_max(S)) * c;
@@ -367,7 +360,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, 
     for (int u = 0; u < 2; ++u) {
       const i4v pb = pack8<T>(S, u);
 #pragma unroll
-      for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(fr.tr(vimg, 16 * u, dn), pb, O[dn]);
+      for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(vf[u * DN + dn], pb, O[dn]);
     }
   }
   l = half_sum(l);
@@ -384,17 +377,17 @@ __global__ __launch_bounds__(kThreads, 1) void k_ga_split(GaArgs a, int rtiles, 
       *reinterpret_cast<f4v*>(jo + (wave * 32 + r32) * OS + 32 * dn + 8 * q + 4 * h) =
           f4v{O[dn][4 * q], O[dn][4 * q + 1], O[dn][4 * q + 2], O[dn][4 * q + 3]};
   __syncthreads();
-  constexpr int PER = D / 8;  // dims of a thread: 8 threads a row
-  const int row = tid >> 3, d0 = (tid & 7) * PER, grow = rt * 32 + row;
+  constexpr int TPR = 64 * NW / 32, PER = D / TPR;  // threads a row, dims a thread
+  const int row = tid / TPR, d0 = (tid % TPR) * PER, grow = rt * 32 + row;
   if (grow >= rows) return;
   float mm = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[0][w][row]);
+  for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sml[0][w][row]);
   float lw = 0.f, acc[PER];
 #pragma unroll
   for (int d = 0; d < PER; ++d) acc[d] = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float mw = sml[0][w][row], f = mw == -INFINITY ? (sml[1][w][row] == 0.f ? 0.f : 1.f)
                                                          : __builtin_amdgcn_exp2f(mw - mm);
     lw += f * sml[1][w][row];
@@ -439,17 +432,33 @@ __global__ __launch_bounds__(kThreads) void k_ga_join(GaArgs a, int rtiles, int 
   if (grow >= rows) return;
   const float* wo = ws + ((int64_t)prob * splits * 32 + row) * D + d;
   const float* wm = ws + (int64_t)units * rtiles * splits * 32 * D + ((int64_t)prob * splits * 32 + row) * 2;
-  float mm = -INFINITY;
-  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, wm[(int64_t)s * 64]);
-  float l = 0.f;
+  // 4 splits' loads in flight at a time; the running maximum rescales what is already there
+  float mm = -INFINITY, l = 0.f;
   f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float ms = wm[(int64_t)s * 64], ls = wm[(int64_t)s * 64 + 1];
-    const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms - mm);
-    l += f * ls;
-    const f4v o = *reinterpret_cast<const f4v*>(wo + (int64_t)s * 32 * D);
+  for (int s0 = 0; s0 < splits; s0 += 4) {
+    float ms[4], ls[4];
+    f4v o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += f * o[i];
+    for (int x = 0; x < 4; ++x) {
+      const int64_t s = min(s0 + x, splits - 1);
+      ms[x] = wm[s * 64];
+      ls[x] = s0 + x < splits ? wm[s * 64 + 1] : 0.f;
+      o[x] = *reinterpret_cast<const f4v*>(wo + s * 32 * D);
+    }
+    const float mn = fmaxf(mm, fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
+    const float corr = mm == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mm - mn);
+    mm = mn;
+    l *= corr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= corr;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (s0 + x >= splits) break;
+      const float f = ms[x] == -INFINITY ? (ls[x] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms[x] - mm);
+      l += f * ls[x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += f * o[x][i];
+    }
   }
   const int b = unit / a.ng, g = unit % a.ng, jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -788,21 +797,24 @@ SplitPlan split_plan(const GaArgs& a) {
   const int64_t tiled = (int64_t)((a.sq + kTileQ - 1) / kTileQ) * a.b * a.np;
   const int64_t rows = (int64_t)(a.np / a.ng) * a.sq, rt = (rows + 31) / 32, probs = rt * a.b * a.ng;
   if (a.p_drop > 0.f || (tiled >= 256 && rows > 64)) return p;
-  const int64_t want = std::max<int64_t>(1, BH_GA_T3 / probs), most = std::max(1, (a.sk + 127) / 128);
+  const int64_t want = std::max<int64_t>(1, 256 / probs), most = std::max(1, (a.sk + kSplitKeys - 1) / kSplitKeys);
   const int64_t s = std::min(want, most);
   p.rtiles = (int)rt;
-  p.chunk = (int)((((int64_t)a.sk + s - 1) / s + 127) / 128 * 128);
+  p.chunk = (int)((((int64_t)a.sk + s - 1) / s + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
   p.splits = (int)(((int64_t)a.sk + p.chunk - 1) / p.chunk);
   return p;
 }
 
-// runs of a key tile's query blocks: enough workgroups for four rounds of the card's 512 places, at least 4
-// blocks of 64 queries each
+// Runs of a key tile's query blocks. 512 workgroups fill the card; under a plain causal mask the first key tiles
+// have most of the work, and twice as many, heaviest first, level that out (8192 causal keys, 8 key heads of 128:
+// backward 1751 us with 2 runs, 2292 with 1, 1767 with 4). Where tiles weigh the same, more than 512 only adds
+// partial sums (4096 keys, window 512, 8 key heads: 192 us with 2 runs, 220 with 4, 206 with 1). A run has at
+// least 2 blocks of 64 queries.
 int dkdv_splits(const GaArgs& a) {
   const int64_t wgs = (int64_t)((a.sk + kTileQ - 1) / kTileQ) * a.b * a.ng;
   const int64_t blocks = ((int64_t)std::min<int64_t>(a.sq, (int64_t)a.window + kTileQ) + 63) / 64 * (a.np / a.ng);
-  const int64_t target = a.causal ? BH_GA_T1 : BH_GA_T2;
-  return (int)std::max<int64_t>(1, std::min(target / wgs, blocks / 4));
+  const int64_t target = a.causal && a.window >= a.sk ? 1024 : 512;
+  return (int)std::max<int64_t>(1, std::min(target / wgs, blocks / 2));
 }
 
 }  // namespace
@@ -816,7 +828,6 @@ int64_t ga_forward_workspace(const GaArgs& a) {
 
 void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
   const SplitPlan p = split_plan(a);
-  const int nx = (a.sq + kTileQ - 1) / kTileQ;
   dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
     using T = typename decltype(t)::type;
     constexpr int D = decltype(dd)::value;
@@ -824,7 +835,7 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
     if (p.splits > 0) {
       if constexpr (!DROP) {
         const int64_t probs = (int64_t)a.b * a.ng * p.rtiles;
-        hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(kThreads), 0, st, a, p.rtiles,
+        hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(64 * kSplitWaves), 0, st, a, p.rtiles,
                            p.splits, p.chunk, ws);
         if (p.splits > 1) {
           constexpr int rpb = kThreads / (D / 4);
@@ -833,6 +844,7 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
         }
       }
     } else {
+      const int nx = (a.sq + kTileQ - 1) / kTileQ;
       hipLaunchKernelGGL((k_ga_fwd<T, D, DROP>), dim3((unsigned)((int64_t)nx * a.b * a.np)), dim3(kThreads), 0, st, a,
                          nx, keep_thresh(a), keep_scale(a));
     }

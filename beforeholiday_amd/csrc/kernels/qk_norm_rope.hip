@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 namespace bh {
 namespace {
@@ -36,32 +37,25 @@ template <typename T> BH_DEVICE void store4(T* p, const float (&r)[8], int at) {
   *reinterpret_cast<t4*>(p) = t4{from_f<T>(r[at]), from_f<T>(r[at + 1]), from_f<T>(r[at + 2]), from_f<T>(r[at + 3])};
 }
 
-// The 4 pairs of a lane: registers i and 4 + i (i < 4) are a pair. With split halves and in the pass-through
-// part, VEC, registers 0..3 and 4..7 are runs of 4 at e0 and e1; interleaved, register 2i / 2i + 1 of the 8 run
-// values are pair i and are put in place after the load.
+// The 4 pairs of a lane. VEC: two runs of 4 values from e0 and e1; with split halves (and in the part that is not
+// rotated) registers i and 4 + i are a pair, interleaved registers 2 i and 2 i + 1 (the runs are neighbours).
 template <bool VEC> struct Slots {
-  int e0, e1;       // VEC: start of the two runs
-  int first, half;  // !VEC: first pair, rot / 2
-  bool inter, live; // live: the lane has a pair below hn / 2
+  int e0, e1;        // VEC: start of the two runs
+  int first, half;   // first pair, rot / 2
   int hn;
-  BH_DEVICE Slots(int c, int hn_, int rot, bool il) : first(4 * c), half(rot >> 1), inter(il), hn(hn_) {
+  bool inter, live;  // live: the lane has a pair below hn / 2
+  BH_DEVICE Slots(int c, int hn_, int rot, bool il) : first(4 * c), half(rot >> 1), hn(hn_), inter(il) {
     live = 8 * c < hn;
-    if (il || 8 * c >= rot) {
-      e0 = 8 * c;
-      e1 = 8 * c + 4;
-    } else {
-      e0 = 4 * c;
-      e1 = half + 4 * c;
-    }
+    const bool halves = !il && 8 * c < rot;
+    e0 = halves ? 4 * c : 8 * c;
+    e1 = halves ? half + 4 * c : 8 * c + 4;
   }
   // element of register k (0..7) on the scalar path; -1: none
   BH_DEVICE int elem(int k) const {
-    const int pair = first + (k & 3), second = k >> 2;
+    const int pair = first + (inter ? k >> 1 : k & 3), second = inter ? k & 1 : k >> 2;
     if (2 * pair >= hn) return -1;
-    if (inter) return 2 * pair + second;
-    return pair < half ? pair + (second ? half : 0) : 2 * pair + second;
+    return !inter && pair < half ? pair + (second ? half : 0) : 2 * pair + second;
   }
-  BH_DEVICE bool swap() const { return inter; }
   template <typename T> BH_DEVICE void load(const T* p, float (&r)[8]) const {
     if (!live) {
 #pragma unroll
@@ -69,14 +63,8 @@ template <bool VEC> struct Slots {
       return;
     }
     if (VEC) {
-      float t[8];
-      load4<T>(p + e0, t, 0);
-      load4<T>(p + e1, t, 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r[i] = inter ? t[2 * i] : t[i];
-        r[4 + i] = inter ? t[2 * i + 1] : t[4 + i];
-      }
+      load4<T>(p + e0, r, 0);
+      load4<T>(p + e1, r, 4);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -88,14 +76,8 @@ template <bool VEC> struct Slots {
   template <typename T> BH_DEVICE void store(T* p, const float (&r)[8]) const {
     if (!live) return;
     if (VEC) {
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        t[inter ? 2 * i : i] = r[i];
-        t[inter ? 2 * i + 1 : 4 + i] = r[4 + i];
-      }
-      store4<T>(p + e0, t, 0);
-      store4<T>(p + e1, t, 4);
+      store4<T>(p + e0, r, 0);
+      store4<T>(p + e1, r, 4);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -106,9 +88,18 @@ template <bool VEC> struct Slots {
   }
 };
 
+// sum over the LPR lanes of a head (8 lanes and more): moves inside 16 lanes are DPP operands of the adds
+template <int CTRL> BH_DEVICE float add_dpp(float v) {
+  const int x = __builtin_bit_cast(int, v);
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, true));
+}
 template <int LPR> BH_DEVICE float row_sum(float v) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  v = add_dpp<0xB1>(v);                  // quad_perm 1 0 3 2
+  v = add_dpp<0x4E>(v);                  // quad_perm 2 3 0 1
+  v = add_dpp<0x141>(v);                 // row_half_mirror
+  if (LPR >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if (LPR >= 32) v += __shfl_xor(v, 16, kWave);
+  if (LPR >= 64) v += __shfl_xor(v, 32, kWave);
   return v;
 }
 
@@ -130,12 +121,18 @@ BH_DEVICE void angles(const QkRopeArgs& a, int t, int b, int first, float (&c)[4
   }
 }
 // pairs turned by +angle (SIGN 1) or -angle (SIGN -1)
-template <int SIGN> BH_DEVICE void turn(float (&r)[8], const float (&c)[4], const float (&s)[4]) {
+template <int SIGN> BH_DEVICE void turn(float (&r)[8], const float (&c)[4], const float (&s)[4], bool inter) {
+  auto pair = [&](int i, float& x, float& y) {
+    const float q = SIGN > 0 ? s[i] : -s[i], u = x, v = y;
+    x = u * c[i] - v * q;
+    y = v * c[i] + u * q;
+  };
+  if (inter) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = r[i], y = r[4 + i], q = SIGN > 0 ? s[i] : -s[i];
-    r[i] = x * c[i] - y * q;
-    r[4 + i] = y * c[i] + x * q;
+    for (int i = 0; i < 4; ++i) pair(i, r[2 * i], r[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair(i, r[i], r[4 + i]);
   }
 }
 template <bool VEC> BH_DEVICE void load_weights(const QkRopeArgs& a, const Slots<VEC>& sl, int k, float (&w)[8]) {
@@ -150,50 +147,72 @@ template <typename T> BH_DEVICE T* row_ptr(const HeadView& v, int t, int b, int 
   return reinterpret_cast<T*>(v.p) + (int64_t)t * v.st + (int64_t)b * v.sb + (int64_t)h * v.sh;
 }
 
-// passes of a token: query heads in groups of HPW, then key heads
+// A token's passes: query heads in groups of HPW (the first nq), then key heads. f gets the operand as a constant,
+// so its weights and sums are registers that are never selected.
+template <typename F> BH_DEVICE void passes(int nq, int p0, int p1, F&& f) {
+  f(std::integral_constant<int, 0>{}, p0, min(p1, nq));
+  f(std::integral_constant<int, 1>{}, max(p0, nq) - nq, p1 - nq);
+}
+
 template <typename T, int LPR, bool VEC, bool NORM>
 __global__ __launch_bounds__(kThreads) void k_qk_rope_fwd(QkRopeArgs a, int ppw) {
   constexpr int HPW = kWave / LPR;
   const int lane = threadIdx.x & (kWave - 1), c = lane % LPR, sub = lane / LPR;
-  const int64_t tok = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int64_t tok = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (tok >= (int64_t)a.s * a.b) return;
   const int t = (int)(tok / a.b), b = (int)(tok - (int64_t)t * a.b);
   const Slots<VEC> sl(c, a.hn, a.rot, a.interleaved);
   const int nq = (a.heads[0] + HPW - 1) / HPW, np = nq + (a.heads[1] + HPW - 1) / HPW;
-  float co[4], si[4], w[2][8];
-  if (a.rot) angles(a, t, b, sl.first, co, si);
-  if (NORM) {
-    load_weights(a, sl, 0, w[0]);
-    load_weights(a, sl, 1, w[1]);
-  }
   const int p0 = blockIdx.y * ppw, p1 = min(p0 + ppw, np);
+  const float inv_n = 1.f / (float)a.hn;
+  float co[4], si[4];
+  if (a.rot) angles(a, t, b, sl.first, co, si);
+  auto run = [&](auto kk, int q0, int q1) {
+    constexpr int k = decltype(kk)::value;
+    if (q0 >= q1) return;
+    float w[8];
+    if (NORM) load_weights(a, sl, k, w);
+    int h = q0 * HPW + sub;
+    const T* x = row_ptr<const T>(a.x[k], t, b, 0) + (int64_t)h * a.x[k].sh;
+    T* y = row_ptr<T>(a.y[k], t, b, 0) + (int64_t)h * a.y[k].sh;
+    const int64_t sx = HPW * a.x[k].sh, sy = HPW * a.y[k].sh;
+    auto head = [&](const T* xp, T* yp, bool on) {
+      float v[8];
+      sl.load(xp, v);
+      if (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+        const float r = rsqrtf(row_sum<LPR>(ss) * inv_n + a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
+      }
+      if (a.rot) turn<1>(v, co, si, sl.inter);
+      if (on) sl.store(yp, v);
+    };
+    int q = q0;
+    const int full = a.heads[k] / HPW;  // passes whose every lane has a head
 #pragma unroll 4
-  for (int p = p0; p < p1; ++p) {
-    const int k = p >= nq, h = (p - (k ? nq : 0)) * HPW + sub;
-    const bool on = h < a.heads[k];
-    float x[8];
-    sl.load(row_ptr<const T>(a.x[k], t, b, on ? h : 0), x);
-    if (NORM) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-      const float r = rsqrtf(row_sum<LPR>(ss) / (float)a.hn + a.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (k ? w[1][i] : w[0][i]);
+    for (; q < min(q1, full); ++q, x += sx, y += sy) head(x, y, true);
+    if (q < q1) {
+      const bool on = q * HPW + sub < a.heads[k];
+      head(on ? x : row_ptr<const T>(a.x[k], t, b, 0), y, on);
     }
-    if (a.rot) turn<1>(x, co, si);
-    if (on) sl.store(row_ptr<T>(a.y[k], t, b, h), x);
-  }
+  };
+  passes(nq, p0, p1, run);
 }
 
 template <typename T, int LPR, bool VEC, bool NORM>
 __global__ __launch_bounds__(kThreads) void k_qk_rope_bwd(QkRopeArgs a, int ppw, float* __restrict__ part) {
   constexpr int HPW = kWave / LPR;
   __shared__ float sh[NORM ? kWaves : 1][NORM ? 2 * 8 * LPR : 1];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, c = lane % LPR, sub = lane / LPR;
+  const int lane = threadIdx.x & (kWave - 1), c = lane % LPR, sub = lane / LPR;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t toks = (int64_t)a.s * a.b;
   const Slots<VEC> sl(c, a.hn, a.rot, a.interleaved);
   const int nq = (a.heads[0] + HPW - 1) / HPW, np = nq + (a.heads[1] + HPW - 1) / HPW;
+  const int p0 = blockIdx.y * ppw, p1 = min(p0 + ppw, np);
+  const float inv_n = 1.f / (float)a.hn;
   float w[2][8], dw[2][8];
   if (NORM) {
     load_weights(a, sl, 0, w[0]);
@@ -201,41 +220,52 @@ __global__ __launch_bounds__(kThreads) void k_qk_rope_bwd(QkRopeArgs a, int ppw,
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.f;
   }
-  const int p0 = blockIdx.y * ppw, p1 = min(p0 + ppw, np);
-  const float inv_n = 1.f / (float)a.hn;
   for (int64_t tok = (int64_t)blockIdx.x * kWaves + wave; tok < toks; tok += (int64_t)gridDim.x * kWaves) {
     const int t = (int)(tok / a.b), b = (int)(tok - (int64_t)t * a.b);
     float co[4], si[4];
     if (a.rot) angles(a, t, b, sl.first, co, si);
-#pragma unroll 2
-    for (int p = p0; p < p1; ++p) {
-      const int k = p >= nq, h = (p - (k ? nq : 0)) * HPW + sub;
-      const bool on = h < a.heads[k];
-      float x[8], g[8];
-      sl.load(row_ptr<const T>(a.dy[k], t, b, on ? h : 0), g);
-      if (NORM) sl.load(row_ptr<const T>(a.x[k], t, b, on ? h : 0), x);
-      if (a.rot) turn<-1>(g, co, si);
-      if (NORM) {
-        float ss = 0.f, gx = 0.f, gw[8];
+    auto run = [&](auto kk, int q0, int q1) {
+      constexpr int k = decltype(kk)::value;
+      if (q0 >= q1) return;
+      const int h = q0 * HPW + sub;
+      const T* x = row_ptr<const T>(a.x[k], t, b, 0) + (int64_t)h * a.x[k].sh;
+      const T* dy = row_ptr<const T>(a.dy[k], t, b, 0) + (int64_t)h * a.dy[k].sh;
+      T* y = row_ptr<T>(a.y[k], t, b, 0) + (int64_t)h * a.y[k].sh;
+      const int64_t sx = HPW * a.x[k].sh, sd = HPW * a.dy[k].sh, sy = HPW * a.y[k].sh;
+      auto head = [&](const T* xp, const T* dp, T* yp, bool on) {
+        float v[8], g[8];
+        sl.load(dp, g);
+        if (NORM) sl.load(xp, v);
+        if (a.rot) turn<-1>(g, co, si, sl.inter);
+        if (NORM) {
+          float ss = 0.f, gx = 0.f, gw[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          gw[i] = g[i] * (k ? w[1][i] : w[0][i]);
-          ss = fmaf(x[i], x[i], ss);
-          gx = fmaf(gw[i], x[i], gx);
-        }
-        ss = row_sum<LPR>(ss);
-        gx = row_sum<LPR>(gx);
-        const float r = rsqrtf(ss * inv_n + a.eps), m = gx * r * inv_n;
+          for (int i = 0; i < 8; ++i) {
+            gw[i] = g[i] * w[k][i];
+            ss = fmaf(v[i], v[i], ss);
+            gx = fmaf(gw[i], v[i], gx);
+          }
+          ss = row_sum<LPR>(ss);
+          gx = row_sum<LPR>(gx);
+          const float r = rsqrtf(ss * inv_n + a.eps), m = gx * r * r * inv_n, keep = on ? r : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float xh = x[i] * r, d = on ? g[i] * xh : 0.f;
-          if (k) dw[1][i] += d;
-          else dw[0][i] += d;
-          g[i] = r * (gw[i] - xh * m);
+          for (int i = 0; i < 8; ++i) {
+            dw[k][i] = fmaf(g[i], v[i] * keep, dw[k][i]);
+            g[i] = r * (gw[i] - v[i] * m);
+          }
         }
+        if (on) sl.store(yp, g);
+      };
+      int q = q0;
+      const int full = a.heads[k] / HPW;
+#pragma unroll 4
+      for (; q < min(q1, full); ++q, x += sx, dy += sd, y += sy) head(x, dy, y, true);
+      if (q < q1) {
+        const bool on = q * HPW + sub < a.heads[k];
+        head(on ? x : row_ptr<const T>(a.x[k], t, b, 0), on ? dy : row_ptr<const T>(a.dy[k], t, b, 0), y, on);
       }
-      if (on) sl.store(row_ptr<T>(a.y[k], t, b, h), g);
-    }
+    };
+    passes(nq, p0, p1, run);
   }
   if (NORM) {
 #pragma unroll
