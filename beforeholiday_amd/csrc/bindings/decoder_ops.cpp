@@ -78,7 +78,7 @@ bh::GaArgs ga_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
     a.lens = lens->data_ptr<int>();
   }
   a.scale = (float)scale;
-  a.p_drop = (float)p;
+  a.p_drop = p;
   a.seed = (uint64_t)seed;
   a.seed_dev = step_seed(seed_dev, q, "grouped attention");
   return a;
@@ -181,7 +181,7 @@ variable_list ga_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tens
   auto delta = at::empty_like(lse);
   a.delta = delta.data_ptr<float>();
   at::Tensor rowh, ws;
-  if (a.p_drop > 0.f) {
+  if (a.p_drop > 0) {
     rowh = at::empty(lse.sizes(), lse.options().dtype(at::kInt));
     a.rowh = reinterpret_cast<uint32_t*>(rowh.data_ptr());
   }
@@ -346,17 +346,23 @@ variable_list rope_bwd(const at::Tensor& dyq, const at::Tensor& dyk, const at::T
   vec = rope_view(dyk, q, "key gradient", a.dy[1]) && vec;
   a.vec = a.vec && vec;
   const auto f32 = q.options().dtype(at::kFloat);
-  at::Tensor dw = a.w[0] ? at::empty({2, q.size(3)}, f32) : at::Tensor();
+  at::Tensor dwq, dwk;
+  if (a.w[0]) {
+    dwq = at::empty(wq->sizes(), wq->options());
+    dwk = at::empty(wk->sizes(), wk->options());
+  }
   if (dq.numel() + dk.numel() == 0) {
-    if (dw.defined()) dw.zero_();
+    if (dwq.defined()) {
+      dwq.zero_();
+      dwk.zero_();
+    }
   } else {
     const int64_t rows = bh::qk_rope_partial_rows(a);
     at::Tensor part = rows ? at::empty({rows * 2 * q.size(3)}, f32) : at::Tensor();
     bh::qk_rope_backward(dtype_code(q.scalar_type()), a, rows ? part.data_ptr<float>() : nullptr,
-                         rows ? dw.data_ptr<float>() : nullptr, stream_for(q));
+                         rows ? dwq.data_ptr() : nullptr, rows ? dwk.data_ptr() : nullptr, stream_for(q));
   }
-  if (!dw.defined()) return {dq, dk, dw, dw};
-  return {dq, dk, dw.select(0, 0).to(wq->scalar_type()), dw.select(0, 1).to(wk->scalar_type())};
+  return {dq, dk, dwq, dwk};
 }
 
 struct QkNormRope : torch::autograd::Function<QkNormRope> {

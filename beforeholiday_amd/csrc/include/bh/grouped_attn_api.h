@@ -21,7 +21,8 @@ struct GaArgs {
   int causal = 0;
   int window = 1 << 30;        // keys a causal query sees, its own included
   const int* lens = nullptr;  // [b] keys of each sequence (device), clamped to 0 .. sk
-  float scale = 1.f, p_drop = 0.f;
+  float scale = 1.f;
+  double p_drop = 0.;
   uint64_t seed = 0;
   const int64_t* seed_dev = nullptr;  // step seed of a captured step (utils/graph_rng.py)
   float* lse = nullptr;               // [b, np, sq] log2-sum-exp2 of the base-2 scaled scores, +inf: no key seen

@@ -120,9 +120,13 @@ BH_DEVICE uint32_t row_hash(uint64_t seed, int bh, int q) {
                mix32((uint32_t)(seed >> 32) ^ ((uint32_t)bh * 0x9E3779B1u) ^ ((uint32_t)q * 0x85EBCA77u)));
 }
 BH_DEVICE uint32_t fold16(uint32_t x) { return x ^ (x >> 16); }
+// the pair's hash before its last fold: keep16(fold16(x), t) is the even key's decision, x < t << 16 the odd one's
 BH_DEVICE uint32_t pair_hash(uint32_t rowh, int k) {
-  return fold16(fold16(rowh + (uint32_t)(k >> 1) * 0x9E3779B9u) * 0x7feb352du);
+  return fold16(rowh + (uint32_t)(k >> 1) * 0x9E3779B9u) * 0x7feb352du;
 }
+BH_DEVICE bool keep16(uint32_t x, uint32_t thresh) { return (uint16_t)x < (uint16_t)thresh; }  // thresh <= 65535
+BH_DEVICE bool keep_even(uint32_t x, uint32_t thresh) { return keep16(fold16(x), thresh); }
+BH_DEVICE bool keep_odd(uint32_t x, uint32_t thresh) { return x < thresh << 16; }
 
 }  // namespace m32
 }  // namespace bh

@@ -37,8 +37,8 @@ struct QkRopeArgs {
 void qk_rope_forward(int dt, const QkRopeArgs& a, hipStream_t st);
 // rows of partial weight-gradient sums (floats: rows * 2 * hn) that the backward needs; 0 without weights
 int64_t qk_rope_partial_rows(const QkRopeArgs& a);
-// dw: [2, hn] fp32 (query, key)
-void qk_rope_backward(int dt, const QkRopeArgs& a, float* partials, float* dw, hipStream_t st);
+// dwq / dwk: [hn] of the weights' dtype
+void qk_rope_backward(int dt, const QkRopeArgs& a, float* partials, void* dwq, void* dwk, hipStream_t st);
 
 // y = Philox4x32-7(counter i / 4, key seed)[i % 4] < thresh ? x * scale : 0
 void counter_dropout(int dt, const void* x, void* y, int64_t n, uint32_t thresh, float scale, uint64_t seed,

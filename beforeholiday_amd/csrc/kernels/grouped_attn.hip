@@ -246,8 +246,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
         ls[(i >> 1) & 3] += p0 + p1;
         if (DROP) {
           const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
-          S[t][i] = (x & 0xffffu) < thresh ? p0 : 0.f;
-          S[t][i + 1] = (x >> 16) < thresh ? p1 : 0.f;
+          S[t][i] = keep_even(x, thresh) ? p0 : 0.f;
+          S[t][i + 1] = keep_odd(x, thresh) ? p1 : 0.f;
         } else {
           S[t][i] = p0;
           S[t][i + 1] = p1;
@@ -564,8 +564,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_
         const float p1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], c, nl));
         if (DROP) {
           const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
-          P[i] = p0 * (((x & 0xffffu) < thresh ? P[i] * kscale : 0.f) - dl);
-          P[i + 1] = p1 * (((x >> 16) < thresh ? P[i + 1] * kscale : 0.f) - dl);
+          P[i] = p0 * ((keep_even(x, thresh) ? P[i] * kscale : 0.f) - dl);
+          P[i + 1] = p1 * ((keep_odd(x, thresh) ? P[i + 1] * kscale : 0.f) - dl);
         } else {
           P[i] = p0 * (P[i] - dl);
           P[i + 1] = p1 * (P[i + 1] - dl);
@@ -613,6 +613,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int s
   const int b = pr.unit / a.ng, g = pr.unit % a.ng;
   const int nk = seq_keys(a, b), off = a.sk - a.sq;
   const int k0 = pr.tile * kTileQ, k0w = k0 + wave * 32, mykey = k0w + r32;
+  const bool odd = mykey & 1;
   const Frag<D> fr(lane);
   char* const vtile = smem + 2 * BUF + wave * 32 * RB;  // this wave's 32 keys
   i4v kf[KS], vf[VLDS ? 1 : KS];
@@ -677,19 +678,32 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int s
       }
       if (ml) mask_lo(S, mykey - off - qb - 4 * h - 32 * t);
       if (mh) mask_hi(S, mykey - off + a.window - 1 - qb - 4 * h - 32 * t);
+      // Two neighbouring keys share a hash: the even lane takes the pair's for the first 16 queries, the odd one for
+      // the other 16, and they swap.
+      uint32_t hash[16];
+      if (DROP) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const i4v r4 = *reinterpret_cast<const i4v*>(lp + 128 + 32 * t + 8 * q + 4 * h + (odd ? 16 : 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t mine = pair_hash((uint32_t)r4[e], mykey);
+            const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0xB1, 0xf, 0xf, true);
+            hash[4 * q + e] = odd ? other : mine;
+            hash[8 + 4 * q + e] = odd ? mine : other;
+          }
+        }
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float* at4 = lp + 32 * t + 8 * q + 4 * h;
         const f4v l4 = *reinterpret_cast<const f4v*>(at4), d4 = *reinterpret_cast<const f4v*>(at4 + 64);
-        i4v r4 = i4v{0, 0, 0, 0};
-        if (DROP) r4 = *reinterpret_cast<const i4v*>(at4 + 128);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * q + e;
           const float p = __builtin_amdgcn_exp2f(fmaf(S[i], c, -l4[e]));
           if (DROP) {
-            const uint32_t x = pair_hash((uint32_t)r4[e], mykey);
-            const float kk = ((mykey & 1) ? (x >> 16) : (x & 0xffffu)) < thresh ? kscale : 0.f;
+            const float kk = keep16(fold16(hash[i]) >> (odd ? 16 : 0), thresh) ? kscale : 0.f;
             S[i] = p * kk;
             P[i] = p * (P[i] * kk - d4[e]);
           } else {
@@ -786,8 +800,10 @@ template <typename F> void dispatch(int dt, int hn, bool drop, F&& f) {
   }
 }
 // keep where a 16-bit hash is below this: floor((1 - p) 2^16)
-uint32_t keep_thresh(const GaArgs& a) { return (uint32_t)std::min(65536.0, (1.0 - (double)a.p_drop) * 65536.0); }
-float keep_scale(const GaArgs& a) { return a.p_drop < 1.f ? 1.f / (1.f - a.p_drop) : 0.f; }
+uint32_t keep_thresh(const GaArgs& a) { return (uint32_t)std::min(65536.0, (1.0 - a.p_drop) * 65536.0); }
+// whether any weight is dropped: a threshold of 2^16 keeps all (and would not fit the kernels' 16-bit compare)
+bool drops(const GaArgs& a) { return a.p_drop > 0. && keep_thresh(a) < 65536u; }
+float keep_scale(const GaArgs& a) { return (float)(1.0 / (1.0 - a.p_drop)); }
 
 struct SplitPlan {
   int rtiles = 0, splits = 0, chunk = 0;  // splits == 0: the tiled forward
@@ -796,7 +812,7 @@ SplitPlan split_plan(const GaArgs& a) {
   SplitPlan p;
   const int64_t tiled = (int64_t)((a.sq + kTileQ - 1) / kTileQ) * a.b * a.np;
   const int64_t rows = (int64_t)(a.np / a.ng) * a.sq, rt = (rows + 31) / 32, probs = rt * a.b * a.ng;
-  if (a.p_drop > 0.f || (tiled >= 256 && rows > 64)) return p;
+  if (drops(a) || (tiled >= 256 && rows > 64)) return p;
   const int64_t want = std::max<int64_t>(1, 256 / probs), most = std::max(1, (a.sk + kSplitKeys - 1) / kSplitKeys);
   const int64_t s = std::min(want, most);
   p.rtiles = (int)rt;
@@ -828,7 +844,7 @@ int64_t ga_forward_workspace(const GaArgs& a) {
 
 void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
   const SplitPlan p = split_plan(a);
-  dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
+  dispatch(dt, a.hn, drops(a), [&](auto t, auto dd, auto drop) {
     using T = typename decltype(t)::type;
     constexpr int D = decltype(dd)::value;
     constexpr bool DROP = decltype(drop)::value;
@@ -859,7 +875,7 @@ int64_t ga_backward_workspace(const GaArgs& a) {
 
 void ga_backward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
   const int nq = (a.sq + kTileQ - 1) / kTileQ, nkt = (a.sk + kTileQ - 1) / kTileQ, splits = dkdv_splits(a);
-  dispatch(dt, a.hn, a.p_drop > 0.f, [&](auto t, auto dd, auto drop) {
+  dispatch(dt, a.hn, drops(a), [&](auto t, auto dd, auto drop) {
     using T = typename decltype(t)::type;
     constexpr int D = decltype(dd)::value;
     constexpr bool DROP = decltype(drop)::value;

@@ -293,11 +293,27 @@ __global__ __launch_bounds__(kThreads) void k_qk_rope_bwd(QkRopeArgs a, int ppw,
   }
 }
 
-// dw[c] = sum over the partial rows, in order: 16 lanes of rows per column, joined through LDS
-__global__ __launch_bounds__(1024) void k_qk_rope_dw(const float* __restrict__ part, int64_t rows, int64_t n,
-                                                     float* __restrict__ dw) {
-  __shared__ float sh[kColsumLanes][64];
-  colsum_partials_block<float>(part, rows, n, dw, sh);
+// Weight gradients of the query (blockIdx.y 0) and the key (1): sums over the partial rows, each column by 16 lanes
+// that take every 16th row, joined in order through LDS. A block has 64 columns.
+template <typename W>
+__global__ __launch_bounds__(1024) void k_qk_rope_dw(const float* __restrict__ part, int rows, int hn, W* __restrict__ dwq,
+                                                     W* __restrict__ dwk) {
+  __shared__ float sh[16][64];
+  const int col = threadIdx.x & 63, lane = threadIdx.x >> 6, c = blockIdx.x * 64 + col;
+  const float* p = part + (int64_t)blockIdx.y * hn + c;
+  float acc = 0.f;
+  if (c < hn) {
+#pragma unroll 8
+    for (int r = lane; r < rows; r += 16) acc += p[(int64_t)r * 2 * hn];
+  }
+  sh[lane][col] = acc;
+  __syncthreads();
+  if (lane == 0 && c < hn) {
+    float t = 0.f;
+#pragma unroll
+    for (int l = 0; l < 16; ++l) t += sh[l][col];
+    (blockIdx.y ? dwk : dwq)[c] = from_f<W>(t);
+  }
 }
 
 inline void check_launch(const char* what) {
@@ -367,7 +383,7 @@ int64_t qk_rope_partial_rows(const QkRopeArgs& a) {
   return p.gx * p.chunks;
 }
 
-void qk_rope_backward(int dt, const QkRopeArgs& a, float* partials, float* dw, hipStream_t st) {
+void qk_rope_backward(int dt, const QkRopeArgs& a, float* partials, void* dwq, void* dwk, hipStream_t st) {
   const bool norm = a.w[0] != nullptr;
   const Plan p = plan(a, norm);
   dispatch(dt, a, [&](auto t, auto lpr, auto vec, auto nn) {
@@ -375,9 +391,18 @@ void qk_rope_backward(int dt, const QkRopeArgs& a, float* partials, float* dw, h
                                       decltype(nn)::value>),
                        dim3((unsigned)p.gx, (unsigned)p.chunks), dim3(kThreads), 0, st, a, p.ppw, partials);
   });
-  if (norm)
-    hipLaunchKernelGGL(k_qk_rope_dw, dim3((unsigned)((2 * a.hn + 63) / 64)), dim3(1024), 0, st, partials,
-                       p.gx * p.chunks, (int64_t)2 * a.hn, dw);
+  if (norm) {
+    const dim3 grid((unsigned)((a.hn + 63) / 64), 2);
+    const int rows = (int)(p.gx * p.chunks);
+    auto sums = [&](auto w) {
+      using W = typename decltype(w)::type;
+      hipLaunchKernelGGL((k_qk_rope_dw<W>), grid, dim3(1024), 0, st, partials, rows, a.hn, reinterpret_cast<W*>(dwq),
+                         reinterpret_cast<W*>(dwk));
+    };
+    if (a.w_dt == kF16) sums(TypeTag<f16>{});
+    else if (a.w_dt == kBF16) sums(TypeTag<bf16>{});
+    else sums(TypeTag<float>{});
+  }
   check_launch("qk_norm_rope backward");
 }
 
