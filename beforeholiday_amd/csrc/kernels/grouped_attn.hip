@@ -486,7 +486,7 @@ template <typename T> BH_DEVICE float dot8(i4v x, i4v y, float acc) {
 // with its rounding's rest: where few keys carry a query, dP - delta cancels and the rounding of O alone would
 // be a good part of dS (GPT-2-medium's shape: error of dQ 2.5e-3 instead of 2.35e-3, dS rounding included).
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_t thresh, float kscale) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void k_ga_dq(GaArgs a, int nx, uint32_t thresh, float kscale) {
   constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -595,17 +595,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dq(GaArgs a, int nx, uint32_
 // r query heads of the group, so the gradients of shared heads are summed in the accumulators (no atomics, one
 // order). S = Q K^T and dP = dO V^T from row fragments, P and dS feed dV^T = dO^T P and dK^T = Q^T dS from the
 // accumulators. L, delta and the row hashes of a block ride along.
-// Registers decide the shape: at D = 128 the accumulators take 128 of the 256 that two waves a SIMD leave, so V
-// is read from LDS again each block (K stays in registers) and blocks are 32 queries; at D = 64 both stay in
-// registers and blocks are 64.
+// Registers decide the shape: K stays in registers, V is read from LDS again for every block. At D = 128 the
+// accumulators take 128 of the 256 registers that two waves a SIMD leave (with V in registers 34 spilled, and
+// 8192 causal keys took 2.70 ms instead of 1.05); at D = 64 it makes room for a third wave (GPT-2-medium's shape
+// with dropout, dQ + dK / dV: 124 us, 129 with V in registers and two waves). Blocks are 32 queries at D = 128
+// (LDS for two workgroups a CU), 64 at D = 64.
 // The blocks of a key tile are cut into `splits` runs (few key tiles, or a causal mask that gives the first
 // tiles most of the work); their fp32 sums then meet in k_ga_dkdv_join, in order.
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int splits, uint32_t thresh, float kscale,
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void k_ga_dkdv(GaArgs a, int nx, int splits, uint32_t thresh, float kscale,
                                                          float* __restrict__ ws) {
   constexpr int RB = 2 * D, QB = D == 64 ? 64 : 32, IMG = QB * RB, KS = D / 16, DN = D / 32, BUF = 2 * IMG + 3 * 256;
-  constexpr bool VLDS = D == 128;
-  __shared__ __attribute__((aligned(16))) char smem[2 * BUF + (VLDS ? kTileQ * RB : 0)];
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF + kTileQ * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const int r = a.np / a.ng;
@@ -616,13 +617,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int s
   const bool odd = mykey & 1;
   const Frag<D> fr(lane);
   char* const vtile = smem + 2 * BUF + wave * 32 * RB;  // this wave's 32 keys
-  i4v kf[KS], vf[VLDS ? 1 : KS];
+  i4v kf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     kf[s] = load_frag<T>(at<const T>(a.k, b, g), a.k.st, mykey, nk, 16 * s + 8 * h, a.hn);
-    const i4v v = load_frag<T>(at<const T>(a.v, b, g), a.v.st, mykey, nk, 16 * s + 8 * h, a.hn);
-    if (VLDS) *reinterpret_cast<i4v*>(vtile + (fr.r0 ^ (s << 5))) = v;
-    else vf[VLDS ? 0 : s] = v;
+    *reinterpret_cast<i4v*>(vtile + (fr.r0 ^ (s << 5))) =
+        load_frag<T>(at<const T>(a.v, b, g), a.v.st, mykey, nk, 16 * s + 8 * h, a.hn);
   }
   const float c = a.scale * kLog2e;
   f16v dK[DN], dV[DN];
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_dkdv(GaArgs a, int nx, int s
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         S = Mfma<T>::run(fr.row(qimg, 32 * t, s), kf[s], S);
-        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), VLDS ? fr.row(vtile, 0, s) : vf[VLDS ? 0 : s], P);  // dP
+        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), fr.row(vtile, 0, s), P);  // dP
       }
       if (ml) mask_lo(S, mykey - off - qb - 4 * h - 32 * t);
       if (mh) mask_hi(S, mykey - off + a.window - 1 - qb - 4 * h - 32 * t);
