@@ -38,6 +38,13 @@ bool use_vec(int n2, std::initializer_list<at::Tensor> ts) {
 int wc(const at::Tensor& w) { return w.defined() ? dtype_code(w.scalar_type()) : -1; }
 const void* wp(const at::Tensor& w) { return w.defined() ? w.data_ptr() : nullptr; }
 
+// weights elsewhere (a module that was never moved to the GPU) would be read by the kernels as GPU memory
+void check_weights(const at::Tensor& x, int n2, std::initializer_list<at::Tensor> ws) {
+  for (const auto& w : ws)
+    TORCH_CHECK(!w.defined() || (w.device() == x.device() && w.numel() == n2), "layer_norm: weight / bias must have ", n2,
+                " elements on ", x.device(), ", got ", w.sizes(), " on ", w.device());
+}
+
 // forward: returns (output, mean, invvar); rms -> mean undefined
 std::vector<at::Tensor> fwd_impl(at::Tensor input, at::IntArrayRef shape, at::Tensor gamma, at::Tensor beta,
                                  double eps, bool rms, bool mixed) {
@@ -46,6 +53,7 @@ std::vector<at::Tensor> fwd_impl(at::Tensor input, at::IntArrayRef shape, at::Te
   if (gamma.defined()) gamma = gamma.contiguous();
   if (beta.defined()) beta = beta.contiguous();
   auto d = dims_of(input, shape);
+  check_weights(input, d.n2, {gamma, beta});
   auto st = (mixed && gamma.defined()) ? gamma.scalar_type() : input.scalar_type();
   auto out = at::empty_like(input, input.options().dtype(st));
   std::vector<int64_t> stat_shape(input.sizes().begin(), input.sizes().end() - shape.size());
@@ -70,6 +78,7 @@ std::vector<at::Tensor> bwd_impl(at::Tensor dout, at::Tensor mean, at::Tensor in
   if (gamma.defined()) gamma = gamma.contiguous();
   if (beta.defined()) beta = beta.contiguous();
   auto d = dims_of(xin, shape);
+  check_weights(xin, d.n2, {gamma, beta});
   auto dx = at::empty_like(xin);
   if (dresid.defined()) {
     dresid = dresid.contiguous();
