@@ -26,7 +26,8 @@ from ..normalization import ResidualGradLink
 from ..ops import fused_dense as _fd
 from ..transformer import parallel_state, tensor_parallel
 from ..transformer.enums import AttnMaskType, AttnType, LayerType, ModelType
-from ..transformer.functional import FusedScaleMaskSoftmax
+from ..transformer.functional import (FusedScaleMaskSoftmax, fused_dropout, fused_grouped_attention, fused_qk_norm_rope,
+                                      rotary_tables)
 from ..transformer.layers import FusedLayerNorm as LayerNorm
 from ..transformer.utils import divide
 
@@ -62,6 +63,31 @@ class TransformerConfig:
     activations_checkpoint_num_layers: int = 1
     pooler: bool = False
     bert_binary_head: bool = True
+    # decoder attention options (causal self-attention; any of them selects transformer.functional's
+    # fused_grouped_attention, fp16 / bf16 on the GPU, head sizes in steps of 8 up to 128)
+    num_query_groups: Optional[int] = None  # key / value heads (None: as many as query heads)
+    qk_norm: bool = False  # RMS norm of every query and key head
+    position_embedding_type: str = "learned"  # "learned" | "rope" (rotation by the token's index, no learned table)
+    rotary_percent: float = 1.0  # leading share of a head that is rotated
+    rotary_base: float = 10000.0
+    rotary_interleaved: bool = False
+    attention_window: Optional[int] = None  # keys a query sees, its own included
+    grouped_attention: bool = False  # fused_grouped_attention without any of the options above
+    counter_dropout: bool = False  # embedding dropout by fused_dropout (no stored mask, replayable in a HIP graph)
+
+    @property
+    def decoder_attention(self) -> bool:
+        """Whether causal self-attention runs on fused_grouped_attention."""
+        return (self.grouped_attention or self.qk_norm or self.position_embedding_type == "rope"
+                or self.attention_window is not None or self.query_groups != self.num_attention_heads)
+
+    @property
+    def query_groups(self) -> int:
+        return self.num_query_groups or self.num_attention_heads
+
+    @property
+    def rotary_dim(self) -> int:
+        return int(self.kv_channels * self.rotary_percent) // 2 * 2
 
     def __post_init__(self):
         if self.ffn_hidden_size is None:
@@ -69,6 +95,15 @@ class TransformerConfig:
         if self.kv_channels is None:
             assert self.hidden_size % self.num_attention_heads == 0
             self.kv_channels = self.hidden_size // self.num_attention_heads
+        if self.num_query_groups is not None and (self.num_query_groups < 1 or
+                                                  self.num_attention_heads % self.num_query_groups):
+            raise ValueError(f"num_query_groups={self.num_query_groups} does not divide {self.num_attention_heads} heads")
+        if self.position_embedding_type not in ("learned", "rope"):
+            raise ValueError(f"position_embedding_type={self.position_embedding_type!r}: expected 'learned' or 'rope'")
+        if self.position_embedding_type == "rope" and not 2 <= self.rotary_dim <= self.kv_channels:
+            raise ValueError(f"rotary_percent={self.rotary_percent} rotates {self.rotary_dim} of {self.kv_channels} values")
+        if self.attention_window is not None and self.attention_window < 1:
+            raise ValueError(f"attention_window={self.attention_window}: a query sees at least its own position")
 
 
 def init_method_normal(sigma):
@@ -340,8 +375,27 @@ class CoreAttention(MegatronModule):
         return ctx.view(sq, b, self.hidden_size_per_partition)
 
 
+_ROTARY_TABLES = {}
+
+
+def _rotary_tables(n_positions, rotary_dim, base, device):
+    """The fp32 angle tables every layer of a model shares (not buffers: a cast of the model must not touch them).
+    They are made once per device on the host and copied before this returns, so any stream may read them."""
+    key = (n_positions, rotary_dim, base, device)
+    if key not in _ROTARY_TABLES:
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("rotary tables: run one step of the model before capturing it")
+        _ROTARY_TABLES[key] = tuple(t.to(device) for t in rotary_tables(n_positions, rotary_dim, base, "cpu"))
+    return _ROTARY_TABLES[key]
+
+
 class ParallelAttention(MegatronModule):
-    """Self-attention (fused QKV projection) or cross-attention; output projection row parallel."""
+    """Self-attention (fused QKV projection) or cross-attention; output projection row parallel.
+
+    With ``config.decoder_attention`` causal self-attention runs on fused_grouped_attention, after
+    fused_qk_norm_rope where the configuration norms or rotates. Fewer key heads than query heads: the
+    projections are ``query`` and ``key_value`` (as in cross-attention), so a tensor-parallel rank holds whole
+    groups; rotary positions are the token indices 0 .. s - 1."""
 
     def __init__(self, config: TransformerConfig, init_method, output_layer_init_method, layer_number,
                  attention_type=AttnType.self_attn, attn_mask_type=AttnMaskType.padding):
@@ -356,20 +410,61 @@ class ParallelAttention(MegatronModule):
                       sequence_parallel_enabled=config.sequence_parallel,
                       no_async_tensor_model_parallel_allreduce=config.sequence_parallel,
                       gradient_accumulation_fusion=config.gradient_accumulation_fusion)
-        if attention_type == AttnType.self_attn:
+        self.decoder = config.decoder_attention and attention_type == AttnType.self_attn
+        if self.decoder and attn_mask_type != AttnMaskType.causal:
+            raise ValueError("num_query_groups, qk_norm, rope, attention_window and grouped_attention need a causal mask")
+        groups = config.query_groups if self.decoder else config.num_attention_heads
+        if attention_type == AttnType.self_attn and groups == config.num_attention_heads:
             self.query_key_value = tensor_parallel.ColumnParallelLinear(config.hidden_size, 3 * projection_size,
                                                                         **common)
         else:
             self.query = tensor_parallel.ColumnParallelLinear(config.hidden_size, projection_size, **common)
-            self.key_value = tensor_parallel.ColumnParallelLinear(config.hidden_size, 2 * projection_size, **common)
-        self.core_attention = CoreAttention(config, layer_number, attn_mask_type)
+            self.key_value = tensor_parallel.ColumnParallelLinear(config.hidden_size, 2 * config.kv_channels * groups,
+                                                                  **common)
+        if self.decoder:
+            self.query_groups_per_partition = divide(groups, world)
+            self.attention_window, self.attention_dropout = config.attention_window, config.attention_dropout
+            self.rotary = None
+            if config.position_embedding_type == "rope":
+                self.rotary = (config.max_position_embeddings, config.rotary_dim, config.rotary_base)
+            self.rotary_interleaved = config.rotary_interleaved
+            self.query_norm = self.key_norm = None
+            if config.qk_norm:
+                self.query_norm, self.key_norm = (torch.nn.Parameter(torch.ones(
+                    config.kv_channels, dtype=config.params_dtype, device=_device(config))) for _ in range(2))
+            self.norm_eps = config.layernorm_epsilon
+        else:
+            self.core_attention = CoreAttention(config, layer_number, attn_mask_type)
         self.dense = tensor_parallel.RowParallelLinear(
             projection_size, config.hidden_size, input_is_parallel=True, init_method=output_layer_init_method,
             skip_bias_add=True, params_dtype=config.params_dtype, use_cpu_initialization=config.use_cpu_initialization,
             sequence_parallel_enabled=config.sequence_parallel,
             gradient_accumulation_fusion=config.gradient_accumulation_fusion)
 
+    def _decoder_forward(self, hidden_states):
+        np_, hn = self.num_attention_heads_per_partition, self.hidden_size_per_attention_head
+        ng = self.query_groups_per_partition
+        if ng == np_:
+            mixed, _ = self.query_key_value(hidden_states)
+            q, k, v = mixed.view(*mixed.shape[:-1], np_, 3 * hn).split(hn, -1)
+        else:
+            q, _ = self.query(hidden_states)
+            q = q.view(*q.shape[:-1], np_, hn)
+            kv, _ = self.key_value(hidden_states)
+            k, v = kv.view(*kv.shape[:-1], ng, 2 * hn).split(hn, -1)
+        if self.rotary is not None or self.query_norm is not None:
+            wq, wk = self.query_norm, self.key_norm
+            if wq is not None:  # replicated over the ranks, each of which sees its own heads
+                wq, wk = (tensor_parallel.copy_to_tensor_model_parallel_region(w) for w in (wq, wk))
+            tables = (None, None) if self.rotary is None else _rotary_tables(*self.rotary, q.device)
+            q, k = fused_qk_norm_rope(q, k, wq, wk, *tables, eps=self.norm_eps, interleaved=self.rotary_interleaved)
+        ctx = fused_grouped_attention(q, k, v, causal=True, window=self.attention_window,
+                                      dropout_p=self.attention_dropout, training=self.training)
+        return self.dense(ctx.view(*ctx.shape[:2], np_ * hn))
+
     def forward(self, hidden_states, attention_mask, encoder_output=None):
+        if self.decoder:
+            return self._decoder_forward(hidden_states)
         np_, hn = self.num_attention_heads_per_partition, self.hidden_size_per_attention_head
         if self.attention_type == AttnType.self_attn:
             mixed, _ = self.query_key_value(hidden_states)
@@ -526,7 +621,8 @@ class ParallelTransformer(MegatronModule):
 
 
 class Embedding(MegatronModule):
-    """word (vocab parallel) + position (+ tokentype) embeddings, dropout; [b, s] -> [s, b, h]."""
+    """word (vocab parallel) + learned position (+ tokentype) embeddings, dropout; [b, s] -> [s, b, h]. With rotary
+    positions there is no position table and ``position_ids`` is not read."""
 
     def __init__(self, config: TransformerConfig, init_method, num_tokentypes=0):
         super().__init__()
@@ -539,9 +635,12 @@ class Embedding(MegatronModule):
             config.vocab_size, config.hidden_size, init_method=init_method, params_dtype=config.params_dtype,
             use_cpu_initialization=config.use_cpu_initialization)
         dev = None if config.use_cpu_initialization or not torch.cuda.is_available() else torch.cuda.current_device()
-        self.position_embeddings = torch.nn.Embedding(config.max_position_embeddings, config.hidden_size,
-                                                      dtype=config.params_dtype, device=dev)
-        init_method(self.position_embeddings.weight)
+        if config.position_embedding_type == "learned":
+            self.position_embeddings = torch.nn.Embedding(config.max_position_embeddings, config.hidden_size,
+                                                          dtype=config.params_dtype, device=dev)
+            init_method(self.position_embeddings.weight)
+        else:
+            self.position_embeddings = None
         if num_tokentypes > 0:
             self.tokentype_embeddings = torch.nn.Embedding(num_tokentypes, config.hidden_size,
                                                            dtype=config.params_dtype, device=dev)
@@ -549,9 +648,12 @@ class Embedding(MegatronModule):
         else:
             self.tokentype_embeddings = None
         self.embedding_dropout = torch.nn.Dropout(config.hidden_dropout)
+        self.counter_dropout = config.counter_dropout
 
     def forward(self, input_ids, position_ids, tokentype_ids=None):
-        emb = self.word_embeddings(input_ids) + _fd.embedding(position_ids, self.position_embeddings.weight)
+        emb = self.word_embeddings(input_ids)
+        if self.position_embeddings is not None:
+            emb = emb + _fd.embedding(position_ids, self.position_embeddings.weight)
         if tokentype_ids is not None:
             assert self.tokentype_embeddings is not None
             emb = emb + _fd.embedding(tokentype_ids, self.tokentype_embeddings.weight)
@@ -560,6 +662,9 @@ class Embedding(MegatronModule):
             emb = emb.float()
         if self.sequence_parallel:
             emb = tensor_parallel.scatter_to_sequence_parallel_region(emb)
+        if self.counter_dropout:
+            return fused_dropout(emb, self.embedding_dropout.p, self.training, model_parallel=self.sequence_parallel)
+        if self.sequence_parallel:
             with tensor_parallel.get_cuda_rng_tracker().fork():
                 return self.embedding_dropout(emb)
         return self.embedding_dropout(emb)

@@ -1,0 +1,228 @@
+"""The transformer LM's decoder attention options (grouped heads, query / key norm, rotary positions, window, counter-based
+embedding dropout): fused_dropout -> fused_qk_norm_rope -> fused_grouped_attention run together as a model runs them."""
+import pytest
+import torch
+
+from tests._dist import run_distributed
+
+OPTS = dict(num_query_groups=2, qk_norm=True, position_embedding_type="rope", rotary_percent=0.5, attention_window=5)
+
+
+def _cfg(**kw):
+    from beforeholiday_amd.models import TransformerConfig
+    base = dict(hidden_size=32, num_layers=2, num_attention_heads=4, vocab_size=64, max_position_embeddings=16,
+                hidden_dropout=0.0, attention_dropout=0.0, params_dtype=torch.float64, use_cpu_initialization=True,
+                masked_softmax_fusion=False)
+    base.update(kw)
+    return TransformerConfig(**base)
+
+
+def _run(cfg, tokens, labels, device="cpu"):
+    from beforeholiday_amd.models import GPTModel, finalize_model_grads
+    torch.manual_seed(7)
+    model = GPTModel(cfg).to(device)
+    for layer in model.language_model.encoder.layers:  # norm weights that do something
+        if layer.self_attention.query_norm is not None:
+            with torch.no_grad():
+                layer.self_attention.query_norm.copy_(torch.linspace(0.5, 1.5, cfg.kv_channels))
+                layer.self_attention.key_norm.copy_(torch.linspace(1.5, 0.7, cfg.kv_channels))
+    loss = model(tokens.to(device), None, None, labels=labels.to(device))
+    loss.float().mean().backward() if device != "cpu" else loss.mean().backward()
+    finalize_model_grads(model)
+    return model, loss.detach()
+
+
+def _single(fn):
+    from beforeholiday_amd.transformer import parallel_state as ps
+    from beforeholiday_amd.transformer import tensor_parallel
+    ps.initialize_model_parallel(1, 1, default_backend="gloo")
+    tensor_parallel.model_parallel_cuda_manual_seed(123)
+    try:
+        return fn()
+    finally:
+        ps.destroy_model_parallel()
+
+
+def _plain_layer(attn, x, cfg):
+    """ParallelAttention written out: projections, RMS norm, rotation, windowed causal softmax, output projection."""
+    s, b, _ = x.shape
+    np_, ng, hn = cfg.num_attention_heads, cfg.query_groups, cfg.kv_channels
+    q = (x @ attn.query.weight.t() + attn.query.bias).view(s, b, np_, hn)
+    kv = (x @ attn.key_value.weight.t() + attn.key_value.bias).view(s, b, ng, 2 * hn)
+    k, v = kv[..., :hn], kv[..., hn:]
+
+    def norm_rotate(t, w):
+        t = t / (t.square().mean(-1, keepdim=True) + cfg.layernorm_epsilon).sqrt() * w
+        h = cfg.rotary_dim // 2
+        ang = torch.arange(s, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(h, dtype=torch.float64) / h)
+        turn = torch.polar(torch.ones_like(ang), ang)[:, None, None]
+        z = torch.complex(t[..., :h], t[..., h:2 * h]) * turn
+        return torch.cat((z.real, z.imag, t[..., 2 * h:]), -1)
+    q, k = norm_rotate(q, attn.query_norm), norm_rotate(k, attn.key_norm)
+    out = []
+    i, j = torch.arange(s)[:, None], torch.arange(s)[None]
+    see = (j <= i) & (i - j < cfg.attention_window)
+    for h in range(np_):
+        sc = torch.einsum("sbd,tbd->bst", q[:, :, h], k[:, :, h // (np_ // ng)]) / hn ** 0.5
+        p = sc.masked_fill(~see, float("-inf")).softmax(-1)
+        out.append(torch.einsum("bst,tbd->sbd", p, v[:, :, h // (np_ // ng)]))
+    return torch.cat(out, -1) @ attn.dense.weight.t()
+
+
+def _layer_worker(rank, world):
+    cfg = _cfg(**OPTS)
+
+    def run():
+        from beforeholiday_amd.models import GPTModel
+        torch.manual_seed(7)
+        model = GPTModel(cfg)
+        attn = model.language_model.encoder.layers[0].self_attention
+        assert not hasattr(attn, "core_attention") and attn.key_value.weight.shape[0] == 2 * 2 * 8
+        assert model.language_model.embedding.position_embeddings is None
+        x = torch.randn(11, 3, 32, dtype=torch.float64, requires_grad=True)
+        got, _ = attn(x, None)
+        want = _plain_layer(attn, x, cfg)
+        torch.testing.assert_close(got, want, rtol=1e-6, atol=1e-9)  # the angle tables are fp32
+        g = torch.randn_like(want)
+        ps = (x, attn.query_norm, attn.key_norm, attn.query.weight, attn.key_value.weight)
+        for a, b in zip(torch.autograd.grad(got, ps, g), torch.autograd.grad(want, ps, g)):
+            torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-8)
+    _single(run)
+
+
+def test_layer_is_its_definition():
+    run_distributed(_layer_worker, 1)
+
+
+def _tp_worker(rank, world, sequence_parallel):
+    from beforeholiday_amd.transformer import parallel_state as ps
+    from beforeholiday_amd.transformer import tensor_parallel
+    torch.manual_seed(0)
+    tokens, labels = torch.randint(0, 64, (2, 8)), torch.randint(0, 64, (2, 8))
+    ref, ref_loss = _single(lambda: _run(_cfg(**OPTS), tokens, labels))
+    ps.initialize_model_parallel(world, 1, default_backend="gloo")
+    tensor_parallel.model_parallel_cuda_manual_seed(123)
+    model, loss = _run(_cfg(sequence_parallel=sequence_parallel, **OPTS), tokens, labels)
+    torch.testing.assert_close(loss, ref_loss)
+    for got, want in zip(model.language_model.encoder.layers, ref.language_model.encoder.layers):
+        got, want = got.self_attention, want.self_attention
+        for name in ("query_norm", "key_norm"):
+            torch.testing.assert_close(getattr(got, name).grad, getattr(want, name).grad)
+        for name in ("query", "key_value"):
+            torch.testing.assert_close(getattr(got, name).weight.grad, getattr(want, name).weight.grad.chunk(world)[rank])
+    ps.destroy_model_parallel()
+
+
+@pytest.mark.parametrize("sequence_parallel", [False, True])
+def test_tensor_parallel_matches_single_rank(sequence_parallel):
+    run_distributed(_tp_worker, 2, sequence_parallel)
+
+
+def _refusal_worker(rank, world):
+    def run():
+        from beforeholiday_amd.models import BertModel
+        for kw in (dict(num_query_groups=3), dict(position_embedding_type="alibi"), dict(attention_window=0),
+                   dict(position_embedding_type="rope", rotary_percent=0.1)):
+            with pytest.raises(ValueError):
+                _cfg(**kw)
+        with pytest.raises(ValueError):
+            BertModel(_cfg(qk_norm=True))
+    _single(run)
+
+
+def test_refusals():
+    run_distributed(_refusal_worker, 1)
+
+
+def _gpu_worker(rank, world):
+    """bf16 on the GPU against the same weights in fp64 on the CPU: loss and every gradient."""
+    def run():
+        torch.manual_seed(0)
+        tokens, labels = torch.randint(0, 64, (3, 150)), torch.randint(0, 64, (3, 150))
+        kw = dict(OPTS, attention_window=40, max_position_embeddings=256, hidden_size=256)
+        ref, ref_loss = _run(_cfg(**kw), tokens, labels)
+        model, loss = _run(_cfg(**dict(kw, params_dtype=torch.bfloat16)), tokens, labels, "cuda")
+        # losses near log 64 from 256 bf16 roundings of 2^-8 half steps that average out
+        torch.testing.assert_close(loss.double().cpu(), ref_loss.double(), rtol=0.02, atol=0.02)
+        got = dict(model.named_parameters())
+        for name, p in ref.named_parameters():
+            g = got[name].grad.double().cpu()
+            assert (g - p.grad).norm() <= 0.06 * p.grad.norm() + 1e-6, name
+    _single(run)
+
+
+@pytest.mark.gpu
+def test_gpu_model_matches_cpu():
+    run_distributed(_gpu_worker, 1)
+
+
+@pytest.mark.gpu
+def test_captured_training_step_with_dropout():
+    """Embedding and attention dropout of the options under device step seeds: a captured step equals the eager step of the
+    same step seed, bit for bit, and draws new masks on the next replay; fp32 is refused."""
+    import torch.distributed as dist
+
+    from beforeholiday_amd.models import GPTModel
+    from beforeholiday_amd.transformer import parallel_state as ps
+    from beforeholiday_amd.transformer import tensor_parallel
+    from beforeholiday_amd.utils import graph_rng
+    import os
+    import tempfile
+
+    assert not dist.is_initialized()
+    path = os.path.join(tempfile.mkdtemp(), "pg")
+    dist.init_process_group("gloo", init_method=f"file://{path}", rank=0, world_size=1)
+    try:
+        ps.initialize_model_parallel(1, 1, default_backend="gloo")
+        tensor_parallel.model_parallel_cuda_manual_seed(123)
+        cfg = dict(OPTS, attention_window=None, max_position_embeddings=256, hidden_size=256, attention_dropout=0.2,
+                   hidden_dropout=0.1, counter_dropout=True, use_cpu_initialization=False)
+        with pytest.raises(ValueError):
+            m = GPTModel(_cfg(**dict(cfg, params_dtype=torch.float32))).cuda()
+            m(torch.zeros(1, 8, dtype=torch.int64, device="cuda"), None, None)
+        torch.manual_seed(3)
+        model = GPTModel(_cfg(**dict(cfg, params_dtype=torch.bfloat16))).cuda()
+        params = [p for p in model.parameters()]
+        tokens = torch.randint(0, 64, (2, 128), device="cuda")
+        graph_rng.enable(seed=5)
+
+        def step():
+            graph_rng.new_step()
+            loss = model(tokens, None, None, labels=tokens).mean()
+            return (loss, *torch.autograd.grad(loss, params))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        losses = []
+        for _ in range(3):
+            at = int(graph_rng.step_seed())
+            graph.replay()
+            torch.cuda.synchronize()
+            replayed = [o.clone() for o in outs]
+            graph_rng.step_seed().fill_(at)
+            for a, b in zip(replayed, step()):
+                assert torch.equal(a, b)
+            losses.append(float(replayed[0]))
+        assert len(set(losses)) == 3
+    finally:
+        graph_rng.disable()
+        ps.destroy_model_parallel()
+        dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_layer_norm_refuses_weights_that_are_not_with_the_input():
+    """A model that was not moved to the GPU whole: its LayerNorm weights are host memory, which no kernel may read."""
+    from beforeholiday_amd.normalization import FusedLayerNorm, FusedRMSNorm
+
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    for norm in (FusedLayerNorm(64), FusedRMSNorm(64)):
+        with pytest.raises(RuntimeError, match="on cuda"):
+            norm(x)
+        assert norm.cuda()(x).shape == x.shape
