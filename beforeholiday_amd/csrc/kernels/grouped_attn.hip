@@ -107,8 +107,10 @@ BH_DEVICE int seq_keys(const GaArgs& a, int b) {
 
 // Problem of a workgroup on a 1-D grid of nx tiles x (b * ng) key heads x per heads. Workgroups go round-robin
 // to the 8 XCDs, each with an L2 of its own, so the tiles and query heads that read one key head's K / V stay
-// on one XCD where the count of key heads allows. tile_major: all problems' tile 0 first (causal: heaviest
-// tiles first, the light ones fill the gaps at the end), else a key head's tiles run together.
+// on one XCD where the count of key heads allows; an XCD takes neighbouring key heads, whose rows lie on
+// different channels of its L2 (2048 x 2500 keys, 16 heads in a fused projection: forward 248 us, 258 with every
+// eighth head). tile_major: all problems' tile 0 first (causal: heaviest tiles first, the light ones fill the gaps
+// at the end), else a key head's tiles run together.
 struct Problem {
   int tile, unit, j;
 };
@@ -120,10 +122,10 @@ BH_DEVICE Problem problem(int nx, int units, int per, bool tile_major) {
   if (tile_major) {
     p.tile = slot / (u * per);
     const int rem = slot - p.tile * (u * per);
-    p.unit = rem / per * nxcd + xcd;
+    p.unit = xcd * u + rem / per;
     p.j = rem % per;
   } else {
-    p.unit = slot / (nx * per) * nxcd + xcd;
+    p.unit = xcd * u + slot / (nx * per);
     const int rem = slot % (nx * per);
     p.tile = rem / per;
     p.j = rem % per;
@@ -155,7 +157,13 @@ BH_DEVICE float tile_max(const f16v& s) {
 // 64-key block into one lane pair's registers, so the softmax needs one half-wave exchange and P^T feeds
 // O^T = V^T P^T from the accumulators. The running maximum is only raised when some query's block maximum
 // passes it by more than 2^8 (P <= 256 rounds as well as P <= 1; a wave-uniform vote).
-// K / V blocks arrive by LDS-DMA one block ahead: one barrier a block.
+// K / V blocks arrive by LDS-DMA one block ahead: one barrier a block. Two workgroups a CU (D = 128: 64 KiB of LDS and
+// 219 registers; four at D = 64) run against each other's matrix and exponential phases.
+// 8192 causal bf16 tokens, 32 heads of 128 over 8: 0.55 ms, 1.0 PFLOP/s (a large matrix product reaches 1.3).
+// The matrix unit is busy 46 % of the cycles; without the LDS-DMA 20 % less time, without exponentials 10 %,
+// without LDS reads 17 % (on zeros, which do not throttle the clock). Measured and not kept, same shape: 8 waves on
+// 256 queries 567 us or on two heads of a group 576 us (557 with 4), three buffers 596 us, the scores of the next
+// 32 keys issued by hand between the exponentials of this one 547 us (532).
 template <typename T, int D, bool DROP>
 __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32_t thresh, float kscale) {
   constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
@@ -284,9 +292,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
 // For grids that would leave the card empty (few queries: single tokens against a long cache). The 32 lanes of
 // a tile are packed rows of one key head -- all r query heads of its group x sq queries -- so a group's K / V
 // are read once. Every wave walks its own 32-key blocks through an LDS buffer of its own (no barrier in the
-// loop); eight waves on a CU with one block in flight each keep the memory busy (one block computed while the
-// next is in flight, with half the waves, measured slower: BH_DECODE). The waves join through LDS, the splits
-// through an fp32 workspace.
+// loop); eight waves on a CU with one block in flight each keep the memory busy: 8 tokens against 4099 keys, 32
+// heads over 8, half the keys there, take 15 + 4 us (34 MB of K / V); four waves that compute one block while the
+// next is in flight took 25 + 6 us. The waves join through LDS, the splits through an fp32 workspace. The kernel is
+// bound by the latency of its few dependent steps: 256 workgroups of at most 5 blocks a wave. 512 workgroups
+// took 31 us where 256 took 27, 128 took 29 (all keys there).
 constexpr int kSplitWaves = 8, kSplitKeys = 32 * kSplitWaves;
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk,
