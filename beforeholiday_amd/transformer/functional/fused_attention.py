@@ -97,8 +97,8 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
     Args:
         query: [sq, b, np, hn]; key, value: [sk, b, ng, hn]. np is a multiple of ng; query head j reads key head
             j // (np / ng). Any strides (views of a fused projection output, transposed batch-first tensors);
-            a layout the kernels cannot address is copied. On the GPU fp16 / bf16, hn a multiple of 8 up to 128;
-            on the CPU any floating type and head size.
+            a layout the kernels cannot address is copied (b * heads * hn of 2^24 and more cannot be). On the GPU
+            fp16 / bf16, hn a multiple of 8 up to 128; on the CPU any floating type and head size.
         causal: query i sees keys up to i + sk - sq: the last query is aligned with the last key.
         window: with ``causal``, a query sees at most this many keys, its own position's included.
         key_lengths: int [b]; keys from key_lengths[n] on are not seen and not read (they may hold anything, and
@@ -111,7 +111,9 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
         seed: default: drawn like the other fused attention dropouts (tensor-parallel ranks differ; replayable
             through ``utils.graph_rng``).
 
-    A query that sees no key gives zeros and takes no gradient. Returns [sq, b, np, hn], contiguous."""
+    A query that sees no key gives zeros and takes no gradient. Contents that only key_lengths hides are never read; a
+    NaN or infinity in a value that the causal mask or the window hides may still reach a query (0 * NaN), as in the
+    written-out product. Returns [sq, b, np, hn], contiguous."""
     if window is not None and (not causal or int(window) < 1):
         raise ValueError("fused_grouped_attention: window needs causal=True and must be at least 1")
     if not 0.0 <= dropout_p < 1.0:

@@ -227,6 +227,52 @@ def test_dropout(shape, p, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(5, 130, 3, 4, 2, 64), (200, 200, 3, 128, 64, 64)])
+def test_key_lengths_outside_the_tensor_count_as_its_ends(shape):
+    q, k, v, dout = make(*shape, torch.float16, "cuda")
+    res = []
+    for lens in (torch.tensor([-3, 2 ** 31 - 1, 65], dtype=torch.int32), torch.tensor([-2 ** 40, 2 ** 40, 65]),
+                 torch.tensor([0, shape[1], 65])):
+        out = fused_grouped_attention(q, k, v, causal=True, key_lengths=lens.cuda())
+        res.append((out, *torch.autograd.grad(out, (q, k, v), dout)))
+    for other in res[:2]:
+        for a, b in zip(other, res[2]):
+            assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("sq", [2, 40000])
+def test_offsets_past_32_bits(sq):
+    """Rows 65536 elements apart: the last ones lie 2.6e9 elements (5.2 GB) behind the first."""
+    sk, wide = 40000, 65536
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def pair(s, heads):
+        t = torch.randn(s, 1, heads, 64, device="cuda", generator=g).half()
+        far = torch.zeros(s, wide, device="cuda", dtype=torch.float16)[:, 8:8 + heads * 64].view(s, 1, heads, 64)
+        far.copy_(t)
+        return t.requires_grad_(), far.detach().requires_grad_()
+    (q, qw), (k, kw), (v, vw), (d, dw) = pair(sq, 2), pair(sk, 1), pair(sk, 1), pair(sq, 2)
+    assert kw.stride(0) == wide
+    near = fused_grouped_attention(q, k, v, causal=True, window=700)
+    far = fused_grouped_attention(qw, kw, vw, causal=True, window=700)
+    assert torch.equal(near, far)
+    for a, b in zip(torch.autograd.grad(near, (q, k, v), d.detach()), torch.autograd.grad(far, (qw, kw, vw), dw.detach())):
+        assert torch.equal(a, b)
+    # and the last row against the definition
+    w, e = oracle(q.detach()[-1:], k.detach()[-700:], v.detach()[-700:], fp16=True, u=torch.finfo(torch.float16).eps / 2)[0]
+    within(near[-1:], w, e, "last query")
+
+
+@gpu
+def test_rows_too_far_apart_are_copied_or_refused():
+    q = torch.randn(2, 1, 1, 64, device="cuda").half()
+    far = torch.zeros(2, (1 << 24) + 8, device="cuda", dtype=torch.float16)[:, :64].view(2, 1, 1, 64).copy_(q)
+    assert far.stride(0) >= 1 << 24
+    assert torch.equal(fused_grouped_attention(q, far, far), fused_grouped_attention(q, q, q))
+
+
+@gpu
 def test_garbage_past_key_lengths_is_not_read():
     for shape in ((6, 200, 3, 4, 2, 64), (200, 200, 3, 128, 64, 128)):
         q, k, v, dout = make(*shape, torch.bfloat16, "cuda")
