@@ -133,6 +133,40 @@ BH_DEVICE Problem problem(int nx, int units, int per, bool tile_major) {
   return p;
 }
 
+// Writes a wave's accumulators (32 rows on the lanes, dims in the registers) to rows of D values in memory. Straight
+// from the registers a store instruction would touch 32 rows with 16 bytes each; through LDS of the wave's own it
+// writes whole rows, 16 bytes a lane (forward of 2048 x 2500 keys, 16 heads of 128: 242 -> 197 us; 4096 tokens, window
+// 512: 71 -> 64 us). The backward kernels store from the registers: with this they were 1 to 2 % slower at D = 128, whose
+// loops have no registers to spare, and no faster at D = 64.
+template <typename T, int D> struct RowsOut {
+  static constexpr int DN = D / 32, RS = 2 * D + 16, BYTES = 32 * RS;
+  static constexpr int CH = D / 8, STEP = 64 / CH;  // chunks of 8 values a row, rows a store
+  char* lds;
+  int lane;
+  // value(dn, i): what goes to dim 32 dn + acc_row(i) + 4 h of this lane's row
+  template <typename F> BH_DEVICE void put(F&& value) const {
+    char* at = lds + (lane & 31) * RS + 8 * (lane >> 5);
+#pragma unroll
+    for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        store4<T>(reinterpret_cast<T*>(at) + 32 * dn + 8 * q, value(dn, 4 * q), value(dn, 4 * q + 1),
+                  value(dn, 4 * q + 2), value(dn, 4 * q + 3));
+  }
+  // rows 0 .. rows - 1 to dst + row * st, their first n values
+  BH_DEVICE void flush(T* dst, int64_t st, int rows, int n) const {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // one wave's LDS: its own order is enough
+    const int ch = lane % CH;
+#pragma unroll
+    for (int i = 0; i < 32 / STEP; ++i) {
+      const int row = i * STEP + lane / CH;
+      const i4v v = *reinterpret_cast<const i4v*>(lds + row * RS + ch * 16);
+      if (row < rows && 8 * ch < n) *reinterpret_cast<i4v*>(dst + (int64_t)row * st + 8 * ch) = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+};
+
 // masks the scores of one 32-key (32-query) tile whose register i stands for offset acc_row(i): keeps
 // lo <= offset <= hi
 BH_DEVICE void mask_hi(f16v& s, int hi) {
@@ -272,25 +306,25 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
       }
   }
   l = half_sum(l);
-  if (myq < a.sq) {
-    const float inv = l > 0.f ? (DROP ? kscale : 1.f) / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
-    const int64_t at_o = (int64_t)myq * a.o.st + 4 * h;
-    T* out = at<T>(a.o, b, head) + at_o;
-    T* rest = a.olo ? at<T>(a.o, b, head, a.olo) + at_o : nullptr;
-#pragma unroll
-    for (int dn = 0; dn < DN; ++dn)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (32 * dn + 8 * q < a.hn)
-          store_out<T>(out + 32 * dn + 8 * q, rest ? rest + 32 * dn + 8 * q : nullptr, O[dn][4 * q] * inv,
-                       O[dn][4 * q + 1] * inv, O[dn][4 * q + 2] * inv, O[dn][4 * q + 3] * inv);
-    if (h == 0) a.lse[(int64_t)bh * a.sq + myq] = l == 0.f ? INFINITY : m + __log2f(l);
+  if (h == 0 && myq < a.sq) a.lse[(int64_t)bh * a.sq + myq] = l == 0.f ? INFINITY : m + __log2f(l);
+  const float inv = l > 0.f ? (DROP ? kscale : 1.f) / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+  lds_barrier();  // every wave is done with the blocks
+  const RowsOut<T, D> out{smem + wave * RowsOut<T, D>::BYTES, lane};
+  const int64_t at_o = (int64_t)q0w * a.o.st;
+  out.put([&](int dn, int i) { return O[dn][i] * inv; });
+  out.flush(at<T>(a.o, b, head) + at_o, a.o.st, a.sq - q0w, a.hn);
+  if (a.olo) {
+    out.put([&](int dn, int i) {
+      const float x = O[dn][i] * inv;
+      return x - to_f<T>(from_f<T>(x));
+    });
+    out.flush(at<T>(a.o, b, head, a.olo) + at_o, a.o.st, a.sq - q0w, a.hn);
   }
 }
 
 // ---- forward, keys split over waves and workgroups ---------------------------------------------------------
 // For grids that would leave the card empty (few queries: single tokens against a long cache). The 32 lanes of
-// a tile are packed rows of one key head -- all r query heads of its group x sq queries -- so a group's K / V
+// a tile are packed rows of one key head (all r query heads of its group x sq queries) so a group's K / V
 // are read once. Every wave walks its own 32-key blocks through an LDS buffer of its own (no barrier in the
 // loop); eight waves on a CU with one block in flight each keep the memory busy: 8 tokens against 4099 keys, 32
 // heads over 8, half the keys there, take 15 + 4 us (34 MB of K / V); four waves that compute one block while the
@@ -613,8 +647,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void k_ga_dq(GaArgs a, i
 // The blocks of a key tile are cut into `splits` runs (few key tiles, or a causal mask that gives the first
 // tiles most of the work); their fp32 sums then meet in k_ga_dkdv_join, in order.
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void k_ga_dkdv(GaArgs a, int nx, int splits, uint32_t thresh, float kscale,
-                                                         float* __restrict__ ws) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void k_ga_dkdv(GaArgs a, int nx, int splits, uint32_t thresh,
+                                                                       float kscale, float* __restrict__ ws) {
   constexpr int RB = 2 * D, QB = D == 64 ? 64 : 32, IMG = QB * RB, KS = D / 16, DN = D / 32, BUF = 2 * IMG + 3 * 256;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF + kTileQ * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -733,8 +767,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void k_ga_dkdv(GaArgs a,
       }
     }
   }
-  if (mykey >= a.sk) return;
   const bool real = mykey < nk;  // keys past the sequence's length take zeros, whatever their lanes held
+  if (mykey >= a.sk) return;
   if (splits > 1) {
     float* w = ws + (((int64_t)pr.j * a.b * a.ng + pr.unit) * a.sk + mykey) * (2 * D) + 4 * h;
 #pragma unroll
