@@ -28,7 +28,7 @@ struct GaArgs {
   float* lse = nullptr;               // [b, np, sq] log2-sum-exp2 of the base-2 scaled scores, +inf: no key seen
   void* olo = nullptr;                // what rounding left of o, laid out like o (null: no backward follows)
   // backward scratch, written by the dQ kernel for the dK / dV kernel
-  float* delta = nullptr;    // [b, np, sq] rowsum(dout * o)
+  float* delta = nullptr;    // [b, np, sq] rowsum(dout * o), or its negative where the dK / dV kernel starts from it
   uint32_t* rowh = nullptr;  // [b, np, sq] dropout row hashes (with dropout)
 };
 

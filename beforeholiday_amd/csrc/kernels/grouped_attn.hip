@@ -109,8 +109,8 @@ BH_DEVICE int seq_keys(const GaArgs& a, int b) {
 // to the 8 XCDs, each with an L2 of its own, so the tiles and query heads that read one key head's K / V stay
 // on one XCD where the count of key heads allows; an XCD takes neighbouring key heads, whose rows lie on
 // different channels of its L2 (2048 x 2500 keys, 16 heads in a fused projection: forward 248 us, 258 with every
-// eighth head). tile_major: all problems' tile 0 first (causal: heaviest tiles first, the light ones fill the gaps
-// at the end), else a key head's tiles run together.
+// eighth head, both before rows were stored whole). tile_major: all problems' tile 0 first (causal: heaviest tiles
+// first, the light ones fill the gaps at the end), else a key head's tiles run together.
 struct Problem {
   int tile, unit, j;
 };
@@ -135,9 +135,9 @@ BH_DEVICE Problem problem(int nx, int units, int per, bool tile_major) {
 
 // Writes a wave's accumulators (32 rows on the lanes, dims in the registers) to rows of D values in memory. Straight
 // from the registers a store instruction would touch 32 rows with 16 bytes each; through LDS of the wave's own it
-// writes whole rows, 16 bytes a lane (forward of 2048 x 2500 keys, 16 heads of 128: 242 -> 197 us; 4096 tokens, window
-// 512: 71 -> 64 us). The backward kernels store from the registers: with this they were 1 to 2 % slower at D = 128, whose
-// loops have no registers to spare, and no faster at D = 64.
+// writes whole rows, 16 bytes a lane (forward of 2048 x 2500 keys, 16 heads of 128: 242 -> 197 us; 4096 tokens,
+// window 512: 71 -> 64 us). The backward kernels store from the registers: with this they were 1 to 2 % slower at
+// D = 128, whose loops have no registers to spare, and no faster at D = 64.
 template <typename T, int D> struct RowsOut {
   static constexpr int DN = D / 32, RS = 2 * D + 16, BYTES = 32 * RS;
   static constexpr int CH = D / 8, STEP = 64 / CH;  // chunks of 8 values a row, rows a store
@@ -167,6 +167,18 @@ template <typename T, int D> struct RowsOut {
   }
 };
 
+// Blocks per turn of a loop over a double buffer. At two of them the buffer's index is a constant in the unrolled body,
+// so that LDS addresses are registers made once plus immediates (sq = 8192, 32 heads on 8, D = 128, causal: forward
+// 558 -> 550 us, backward 1759 -> 1732 us). The 64-channel kernels, whose register limits are tighter, lost more than
+// that (forward 36.0 -> 37.6 us, backward 104 -> 122 us at 8 x 1024 x 16 heads).
+template <int D> constexpr int kTurn = D == 128 ? 2 : 1;
+// buffer of block `block`, the `side`th of its turn
+template <int D> BH_DEVICE int buffer_of(int side, int block) { return (kTurn<D> == 2 ? side : block) & 1; }
+
+// dP - delta without a subtraction: dP's products start from -delta (backward of the same case 1790 -> 1759 us). Not
+// where dropout scales dP first, nor at 64 channels, where the 16 registers of the start spill.
+template <int D, bool DROP> constexpr bool kFromDelta = D == 128 && !DROP;
+
 // masks the scores of one 32-key (32-query) tile whose register i stands for offset acc_row(i): keeps
 // lo <= offset <= hi
 BH_DEVICE void mask_hi(f16v& s, int hi) {
@@ -192,7 +204,7 @@ BH_DEVICE float tile_max(const f16v& s) {
 // O^T = V^T P^T from the accumulators. The running maximum is only raised when some query's block maximum
 // passes it by more than 2^8 (P <= 256 rounds as well as P <= 1; a wave-uniform vote).
 // K / V blocks arrive by LDS-DMA one block ahead: one barrier a block. Two workgroups a CU (D = 128: 64 KiB of LDS and
-// 219 registers; four at D = 64) run against each other's matrix and exponential phases.
+// 224 registers; four at D = 64) run against each other's matrix and exponential phases.
 // 8192 causal bf16 tokens, 32 heads of 128 over 8: 0.55 ms, 1.0 PFLOP/s (a large matrix product reaches 1.3).
 // The matrix unit is busy 46 % of the cycles; without the LDS-DMA 20 % less time, without exponentials 10 %,
 // without LDS reads 17 % (on zeros, which do not throttle the clock). Measured and not kept, same shape: 8 waves on
@@ -239,71 +251,76 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
     sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, wave);
   };
   if (nb > 0) stage(kbeg, smem);
-  for (int ib = 0; ib < nb; ++ib) {
-    const int kb = kbeg + ib * kBlk;
-    const char* kimg = smem + (ib & 1) * 2 * IMG;
-    const char* vimg = kimg + IMG;
-    wait_vmcnt<0>();
-    lds_barrier();  // block ib is in LDS, block ib - 1 is read by every wave
-    if (ib + 1 < nb) stage(kb + kBlk, smem + ((ib + 1) & 1) * 2 * IMG);
-    if (q0w >= a.sq) continue;
-    if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
-    f16v S[2];
+  for (int turn = 0; turn < nb; turn += kTurn<D>) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      S[t] = zero16();
+    for (int side = 0; side < kTurn<D>; ++side) {
+      const int ib = turn + side;
+      if (ib >= nb) break;
+      const int kb = kbeg + ib * kBlk;
+      const char* kimg = smem + buffer_of<D>(side, ib) * 2 * IMG;
+      const char* vimg = kimg + IMG;
+      wait_vmcnt<0>();
+      lds_barrier();  // block ib is in LDS, block ib - 1 is read by every wave
+      if (ib + 1 < nb) stage(kb + kBlk, smem + buffer_of<D>(side + 1, ib + 1) * 2 * IMG);
+      if (q0w >= a.sq) continue;
+      if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
+      f16v S[2];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) S[t] = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S[t]);
-    }
-    const bool diag = a.causal && kb + kBlk - 1 > q0w + off;
-    if (diag || kb + kBlk > nk) {
-      const int hi = (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h;
+      for (int t = 0; t < 2; ++t) {
+        S[t] = zero16();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) mask_hi(S[t], hi - 32 * t);
-    }
-    if (a.causal && kb < qlw + off - a.window + 1) {
-      const int lo = pos - a.window + 1 - kb - 4 * h;
+        for (int s = 0; s < KS; ++s) S[t] = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S[t]);
+      }
+      const bool diag = a.causal && kb + kBlk - 1 > q0w + off;
+      if (diag || kb + kBlk > nk) {
+        const int hi = (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) mask_lo(S[t], lo - 32 * t);
-    }
-    const float mx = half_max(fmaxf(tile_max(S[0]), tile_max(S[1]))) * c;
-    if (__any(mx > m + 8.f)) {
-      const float mn = fmaxf(m, mx);
-      const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= corr;
+        for (int t = 0; t < 2; ++t) mask_hi(S[t], hi - 32 * t);
+      }
+      if (a.causal && kb < qlw + off - a.window + 1) {
+        const int lo = pos - a.window + 1 - kb - 4 * h;
 #pragma unroll
-      for (int dn = 0; dn < DN; ++dn)
+        for (int t = 0; t < 2; ++t) mask_lo(S[t], lo - 32 * t);
+      }
+      const float mx = half_max(fmaxf(tile_max(S[0]), tile_max(S[1]))) * c;
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx);
+        const float corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= corr;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) O[dn][i] *= corr;
-      m = mn;
-    }
-    const float nm = m == -INFINITY ? 0.f : -m;
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int dn = 0; dn < DN; ++dn)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+          for (int i = 0; i < 16; ++i) O[dn][i] *= corr;
+        m = mn;
+      }
+      const float nm = m == -INFINITY ? 0.f : -m;
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[t][i], c, nm));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[t][i + 1], c, nm));
-        ls[(i >> 1) & 3] += p0 + p1;
-        if (DROP) {
-          const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
-          S[t][i] = keep_even(x, thresh) ? p0 : 0.f;
-          S[t][i + 1] = keep_odd(x, thresh) ? p1 : 0.f;
-        } else {
-          S[t][i] = p0;
-          S[t][i + 1] = p1;
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(S[t][i], c, nm));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(S[t][i + 1], c, nm));
+          ls[(i >> 1) & 3] += p0 + p1;
+          if (DROP) {
+            const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
+            S[t][i] = keep_even(x, thresh) ? p0 : 0.f;
+            S[t][i + 1] = keep_odd(x, thresh) ? p1 : 0.f;
+          } else {
+            S[t][i] = p0;
+            S[t][i + 1] = p1;
+          }
         }
-      }
-    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const i4v pb = pack8<T>(S[t], u);
+        for (int u = 0; u < 2; ++u) {
+          const i4v pb = pack8<T>(S[t], u);
 #pragma unroll
-        for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(fr.tr(vimg, 32 * t + 16 * u, dn), pb, O[dn]);
-      }
+          for (int dn = 0; dn < DN; ++dn) O[dn] = Mfma<T>::run(fr.tr(vimg, 32 * t + 16 * u, dn), pb, O[dn]);
+        }
+    }
   }
   l = half_sum(l);
   if (h == 0 && myq < a.sq) a.lse[(int64_t)bh * a.sq + myq] = l == 0.f ? INFINITY : m + __log2f(l);
@@ -531,6 +548,7 @@ template <typename T> BH_DEVICE float dot8(i4v x, i4v y, float acc) {
 // be a good part of dS (GPT-2-medium's shape: error of dQ 2.5e-3 instead of 2.35e-3, dS rounding included).
 template <typename T, int D, bool DROP>
 __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void k_ga_dq(GaArgs a, int nx, uint32_t thresh, float kscale) {
+  constexpr bool FROM = kFromDelta<D, DROP>;
   constexpr int RB = 2 * D, IMG = kBlk * RB, KS = D / 16, DN = D / 32;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -562,7 +580,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void k_ga_dq(GaArgs a, i
   dl = half_sum(dl);
   const uint32_t rowh = DROP ? row_hash(eff_seed(a), bh, myq) : 0u;
   if (h == 0 && myq < a.sq) {
-    a.delta[row] = dl;
+    a.delta[row] = FROM ? -dl : dl;
     if (DROP) a.rowh[row] = rowh;
   }
   f16v acc[DN];
@@ -581,45 +599,53 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void k_ga_dq(GaArgs a, i
     sv.issue(V + (int64_t)kb * a.v.st, a.v.st, a.hn, nk - kb, buf + IMG, wave);
   };
   if (nb > 0) stage(kbeg, smem);
-  for (int ib = 0; ib < nb; ++ib) {
-    const int kb = kbeg + ib * kBlk;
-    const char* kimg = smem + (ib & 1) * 2 * IMG;
-    const char* vimg = kimg + IMG;
-    wait_vmcnt<0>();
-    lds_barrier();
-    if (ib + 1 < nb) stage(kb + kBlk, smem + ((ib + 1) & 1) * 2 * IMG);
-    if (q0w >= a.sq) continue;
-    if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
-    const bool mh = (a.causal && kb + kBlk - 1 > q0w + off) || kb + kBlk > nk;
-    const bool ml = a.causal && kb < qlw + off - a.window + 1;
+  f16v start;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f16v S = zero16(), P = zero16();
+  for (int i = 0; i < 16; ++i) start[i] = FROM ? -dl : 0.f;
+  for (int turn = 0; turn < nb; turn += kTurn<D>) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        S = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S);
-        P = Mfma<T>::run(fr.row(vimg, 32 * t, s), df[s], P);  // dP^T
-      }
-      if (mh) mask_hi(S, (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h - 32 * t);
-      if (ml) mask_lo(S, pos - a.window + 1 - kb - 4 * h - 32 * t);
+    for (int side = 0; side < kTurn<D>; ++side) {
+      const int ib = turn + side;
+      if (ib >= nb) break;
+      const int kb = kbeg + ib * kBlk;
+      const char* kimg = smem + buffer_of<D>(side, ib) * 2 * IMG;
+      const char* vimg = kimg + IMG;
+      wait_vmcnt<0>();
+      lds_barrier();
+      if (ib + 1 < nb) stage(kb + kBlk, smem + buffer_of<D>(side + 1, ib + 1) * 2 * IMG);
+      if (q0w >= a.sq) continue;
+      if (a.causal && (kb > qlw + off || kb + kBlk - 1 < q0w + off - a.window + 1)) continue;
+      const bool mh = (a.causal && kb + kBlk - 1 > q0w + off) || kb + kBlk > nk;
+      const bool ml = a.causal && kb < qlw + off - a.window + 1;
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i], c, nl));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], c, nl));
-        if (DROP) {
-          const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
-          P[i] = p0 * ((keep_even(x, thresh) ? P[i] * kscale : 0.f) - dl);
-          P[i + 1] = p1 * ((keep_odd(x, thresh) ? P[i + 1] * kscale : 0.f) - dl);
-        } else {
-          P[i] = p0 * (P[i] - dl);
-          P[i + 1] = p1 * (P[i + 1] - dl);
+      for (int t = 0; t < 2; ++t) {
+        f16v S = zero16(), P = FROM ? start : zero16();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          S = Mfma<T>::run(fr.row(kimg, 32 * t, s), qf[s], S);
+          P = Mfma<T>::run(fr.row(vimg, 32 * t, s), df[s], P);  // dP^T
         }
-      }
+        if (mh) mask_hi(S, (a.causal ? min(pos, nk - 1) : nk - 1) - kb - 4 * h - 32 * t);
+        if (ml) mask_lo(S, pos - a.window + 1 - kb - 4 * h - 32 * t);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const i4v sb = pack8<T>(P, u);
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i], c, nl));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], c, nl));
+          if (DROP) {
+            const uint32_t x = pair_hash(rowh, kb + 32 * t + acc_row(i) + 4 * h);
+            P[i] = p0 * ((keep_even(x, thresh) ? P[i] * kscale : 0.f) - dl);
+            P[i + 1] = p1 * ((keep_odd(x, thresh) ? P[i + 1] * kscale : 0.f) - dl);
+          } else {
+            P[i] = p0 * (FROM ? P[i] : P[i] - dl);
+            P[i + 1] = p1 * (FROM ? P[i + 1] : P[i + 1] - dl);
+          }
+        }
 #pragma unroll
-        for (int dn = 0; dn < DN; ++dn) acc[dn] = Mfma<T>::run(fr.tr(kimg, 32 * t + 16 * u, dn), sb, acc[dn]);
+        for (int u = 0; u < 2; ++u) {
+          const i4v sb = pack8<T>(P, u);
+#pragma unroll
+          for (int dn = 0; dn < DN; ++dn) acc[dn] = Mfma<T>::run(fr.tr(kimg, 32 * t + 16 * u, dn), sb, acc[dn]);
+        }
       }
     }
   }
@@ -695,74 +721,90 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void k_ga_dkdv(GaArgs a,
   };
   int j = nqb ? it0 / nqb : 0, q0 = qbeg + (it0 - j * nqb) * QB;  // head of the group and first query of a block
   if (it0 < it1) stage(j, q0, smem);
-  for (int it = it0; it < it1; ++it) {
-    const int qb = q0;
-    const char* qimg = smem + ((it - it0) & 1) * BUF;
-    const char* dimg = qimg + IMG;
-    const float* lp = reinterpret_cast<const float*>(dimg + IMG);
-    wait_vmcnt<0>();
-    lds_barrier();
-    q0 += QB;
-    if (q0 >= qend) {
-      q0 = qbeg;
-      ++j;
-    }
-    if (it + 1 < it1) stage(j, q0, smem + ((it - it0 + 1) & 1) * BUF);
-    if (k0w >= nk) continue;
-    if (a.causal && (qb + QB - 1 + off < k0w || qb + off - a.window + 1 > k0w + 31)) continue;
-    const bool ml = a.causal && qb + off < k0w + 31;                       // some query precedes some key
-    const bool mh = a.causal && qb + QB - 1 + off - a.window + 1 > k0w;    // some key left the window
+  constexpr bool FROM = kFromDelta<D, DROP>;
+  for (int turn = it0; turn < it1; turn += kTurn<D>) {
 #pragma unroll
-    for (int t = 0; t < QB / 32; ++t) {
-      f16v S = zero16(), P = zero16();
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        S = Mfma<T>::run(fr.row(qimg, 32 * t, s), kf[s], S);
-        P = Mfma<T>::run(fr.row(dimg, 32 * t, s), fr.row(vtile, 0, s), P);  // dP
+    for (int side = 0; side < kTurn<D>; ++side) {
+      const int it = turn + side;
+      if (it >= it1) break;
+      const int qb = q0;
+      const char* qimg = smem + buffer_of<D>(side, it - it0) * BUF;
+      const char* dimg = qimg + IMG;
+      const float* lp = reinterpret_cast<const float*>(dimg + IMG);
+      wait_vmcnt<0>();
+      lds_barrier();
+      q0 += QB;
+      if (q0 >= qend) {
+        q0 = qbeg;
+        ++j;
       }
-      if (ml) mask_lo(S, mykey - off - qb - 4 * h - 32 * t);
-      if (mh) mask_hi(S, mykey - off + a.window - 1 - qb - 4 * h - 32 * t);
-      // Two neighbouring keys share a hash: the even lane takes the pair's for the first 16 queries, the odd one for
-      // the other 16, and they swap.
-      uint32_t hash[16];
-      if (DROP) {
+      if (it + 1 < it1) stage(j, q0, smem + buffer_of<D>(side + 1, it - it0 + 1) * BUF);
+      if (k0w >= nk) continue;
+      if (a.causal && (qb + QB - 1 + off < k0w || qb + off - a.window + 1 > k0w + 31)) continue;
+      const bool ml = a.causal && qb + off < k0w + 31;                       // some query precedes some key
+      const bool mh = a.causal && qb + QB - 1 + off - a.window + 1 > k0w;    // some key left the window
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const i4v r4 = *reinterpret_cast<const i4v*>(lp + 128 + 32 * t + 8 * q + 4 * h + (odd ? 16 : 0));
+      for (int t = 0; t < QB / 32; ++t) {
+        f16v S = zero16(), P = zero16();
+        if (FROM) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f4v d4 = *reinterpret_cast<const f4v*>(lp + 64 + 32 * t + 8 * q + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) P[4 * q + e] = d4[e];
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          S = Mfma<T>::run(fr.row(qimg, 32 * t, s), kf[s], S);
+          P = Mfma<T>::run(fr.row(dimg, 32 * t, s), fr.row(vtile, 0, s), P);  // dP
+        }
+        if (ml) mask_lo(S, mykey - off - qb - 4 * h - 32 * t);
+        if (mh) mask_hi(S, mykey - off + a.window - 1 - qb - 4 * h - 32 * t);
+        // Two neighbouring keys share a hash: the even lane takes the pair's for the first 16 queries, the odd one for
+        // the other 16, and they swap.
+        uint32_t hash[16];
+        if (DROP) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const i4v r4 = *reinterpret_cast<const i4v*>(lp + 128 + 32 * t + 8 * q + 4 * h + (odd ? 16 : 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t mine = pair_hash((uint32_t)r4[e], mykey);
+              const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0xB1, 0xf, 0xf, true);
+              hash[4 * q + e] = odd ? other : mine;
+              hash[8 + 4 * q + e] = odd ? mine : other;
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float* at4 = lp + 32 * t + 8 * q + 4 * h;
+          const f4v l4 = *reinterpret_cast<const f4v*>(at4);
+          f4v d4 = f4v{0.f, 0.f, 0.f, 0.f};
+          if (!FROM) d4 = *reinterpret_cast<const f4v*>(at4 + 64);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t mine = pair_hash((uint32_t)r4[e], mykey);
-            const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0xB1, 0xf, 0xf, true);
-            hash[4 * q + e] = odd ? other : mine;
-            hash[8 + 4 * q + e] = odd ? mine : other;
+            const int i = 4 * q + e;
+            const float p = __builtin_amdgcn_exp2f(fmaf(S[i], c, -l4[e]));
+            if (DROP) {
+              const float kk = keep16(fold16(hash[i]) >> (odd ? 16 : 0), thresh) ? kscale : 0.f;
+              S[i] = p * kk;
+              P[i] = p * (P[i] * kk - d4[e]);
+            } else {
+              S[i] = p;
+              P[i] = p * (FROM ? P[i] : P[i] - d4[e]);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float* at4 = lp + 32 * t + 8 * q + 4 * h;
-        const f4v l4 = *reinterpret_cast<const f4v*>(at4), d4 = *reinterpret_cast<const f4v*>(at4 + 64);
+        for (int u = 0; u < 2; ++u) {
+          const i4v pb = pack8<T>(S, u), sb = pack8<T>(P, u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * q + e;
-          const float p = __builtin_amdgcn_exp2f(fmaf(S[i], c, -l4[e]));
-          if (DROP) {
-            const float kk = keep16(fold16(hash[i]) >> (odd ? 16 : 0), thresh) ? kscale : 0.f;
-            S[i] = p * kk;
-            P[i] = p * (P[i] * kk - d4[e]);
-          } else {
-            S[i] = p;
-            P[i] = p * (P[i] - d4[e]);
+          for (int dn = 0; dn < DN; ++dn) {
+            dV[dn] = Mfma<T>::run(fr.tr(dimg, 32 * t + 16 * u, dn), pb, dV[dn]);
+            dK[dn] = Mfma<T>::run(fr.tr(qimg, 32 * t + 16 * u, dn), sb, dK[dn]);
           }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const i4v pb = pack8<T>(S, u), sb = pack8<T>(P, u);
-#pragma unroll
-        for (int dn = 0; dn < DN; ++dn) {
-          dV[dn] = Mfma<T>::run(fr.tr(dimg, 32 * t + 16 * u, dn), pb, dV[dn]);
-          dK[dn] = Mfma<T>::run(fr.tr(qimg, 32 * t + 16 * u, dn), sb, dK[dn]);
         }
       }
     }
@@ -895,8 +937,8 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
     if (p.splits > 0) {
       if constexpr (!DROP) {
         const int64_t probs = (int64_t)a.b * a.ng * p.rtiles;
-        hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(64 * kSplitWaves), 0, st, a, p.rtiles,
-                           p.splits, p.chunk, ws);
+        hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(64 * kSplitWaves), 0, st, a,
+                           p.rtiles, p.splits, p.chunk, ws);
         if (p.splits > 1) {
           constexpr int rpb = kThreads / (D / 4);
           hipLaunchKernelGGL((k_ga_join<T, D>), dim3((unsigned)((probs * 32 + rpb - 1) / rpb)), dim3(kThreads), 0, st,
