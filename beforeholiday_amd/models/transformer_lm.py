@@ -385,7 +385,8 @@ def _rotary_tables(n_positions, rotary_dim, base, device):
     if key not in _ROTARY_TABLES:
         if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("rotary tables: run one step of the model before capturing it")
-        _ROTARY_TABLES[key] = tuple(t.to(device) for t in rotary_tables(n_positions, rotary_dim, base, "cpu"))
+        with torch.inference_mode(False):  # a model that evaluates first may train afterwards
+            _ROTARY_TABLES[key] = tuple(t.to(device) for t in rotary_tables(n_positions, rotary_dim, base, "cpu"))
     return _ROTARY_TABLES[key]
 
 

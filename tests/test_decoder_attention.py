@@ -151,6 +151,30 @@ def _gpu_worker(rank, world):
     _single(run)
 
 
+def test_tables_made_in_inference_mode_serve_training():
+    from beforeholiday_amd.models import transformer_lm
+    with torch.inference_mode():
+        tables = transformer_lm._rotary_tables(7, 4, 123.0, torch.device("cpu"))
+    assert not any(t.is_inference() for t in tables)  # those cannot be saved for a backward pass
+
+
+def _recompute_worker(rank, world):
+    tokens = torch.arange(12).view(2, 6) % 64
+
+    def run(**kw):
+        model, loss = _single(lambda: _run(_cfg(attention_dropout=0.5, **OPTS, **kw), tokens, tokens))
+        return loss, [p.grad for p in model.parameters()]
+    loss, grads = run()
+    again, regrads = run(activations_checkpoint_method="uniform")
+    assert torch.equal(loss, again)
+    for g, r in zip(grads, regrads):  # the same fp64 operations on the same masks, summed by autograd in its own order
+        torch.testing.assert_close(r, g, rtol=1e-10, atol=1e-12)
+
+
+def test_recomputed_layers_draw_the_same_masks():
+    run_distributed(_recompute_worker, 1)
+
+
 @pytest.mark.gpu
 def test_gpu_model_matches_cpu():
     run_distributed(_gpu_worker, 1)
@@ -226,3 +250,21 @@ def test_layer_norm_refuses_weights_that_are_not_with_the_input():
         with pytest.raises(RuntimeError, match="on cuda"):
             norm(x)
         assert norm.cuda()(x).shape == x.shape
+
+
+def _gpu_inference_first_worker(rank, world):
+    cfg = _cfg(**dict(OPTS, params_dtype=torch.bfloat16, hidden_size=64))
+    tokens = torch.arange(12).view(2, 6) % 64
+
+    def run():
+        from beforeholiday_amd.models import GPTModel
+        model = GPTModel(cfg).cuda()
+        with torch.inference_mode():  # the process's first step: it makes the rotary tables
+            model(tokens.cuda(), None, None, labels=tokens.cuda())
+        return _run(cfg, tokens, tokens, "cuda")[1]
+    assert torch.isfinite(_single(run)).all()
+
+
+@pytest.mark.gpu
+def test_training_after_a_first_step_in_inference_mode():
+    run_distributed(_gpu_inference_first_worker, 1)
