@@ -304,8 +304,8 @@ bh::QkRopeArgs rope_args(const at::Tensor& q, const at::Tensor& k, const c10::op
       a.pos_sb = pos->dim() == 2 ? pos->stride(1) : 0;
       TORCH_CHECK_VALUE(offset == 0, "qk_norm_rope: an offset goes without positions");
     } else {
-      TORCH_CHECK_VALUE(offset >= 0 && offset + q.size(0) <= a.n_pos, "qk_norm_rope: positions ", offset, " .. ",
-                  offset + q.size(0) - 1, " do not fit tables of ", a.n_pos);
+      TORCH_CHECK_VALUE(offset >= 0 && offset <= a.n_pos - q.size(0), "qk_norm_rope: ", q.size(0), " positions from ",
+                        offset, " on do not fit tables of ", a.n_pos);
       a.offset = offset;
     }
   }

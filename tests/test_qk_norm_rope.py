@@ -306,3 +306,13 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(outs, step()):
             assert torch.equal(a, b)
+
+
+@gpu
+def test_offset_near_the_end_of_64_bits_is_refused():
+    q = torch.zeros(2, 1, 1, 8, device="cuda")
+    cos, sin = rotary_tables(4, 8, device="cuda")
+    for offset in (3, 1 << 62, (1 << 63) - 1):
+        with pytest.raises(ValueError):
+            fused_qk_norm_rope(q, q, None, None, cos, sin, offset=offset)
+    fused_qk_norm_rope(q, q, None, None, cos, sin, offset=2)
