@@ -62,7 +62,7 @@ bh::GaArgs ga_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   TORCH_CHECK_VALUE(q.size(3) >= 8 && q.size(3) <= 128 && q.size(3) % 8 == 0,
               "grouped attention: head_dim must be a multiple of 8 up to 128, got ", q.size(3));
   TORCH_CHECK_VALUE(q.size(0) <= kMaxLen && k.size(0) <= kMaxLen, "grouped attention: sequences of up to 2^29 only");
-  TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, "grouped attention: scale must be positive, got ", scale);
+  TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, "grouped attention: scale must be in [1e-30, 1e30], got ", scale);
   TORCH_CHECK_VALUE(p >= 0 && p < 1, "grouped attention: dropout must be in [0, 1), got ", p);
   a.sq = (int)q.size(0); a.b = (int)q.size(1); a.np = (int)q.size(2); a.hn = (int)q.size(3);
   a.sk = (int)k.size(0); a.ng = (int)k.size(2);

@@ -107,7 +107,7 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
         dropout_p: probability of dropping a softmax weight while ``training`` (the rest is scaled by
             1 / (1 - dropout_p)); resolved to 1 / 65536. The mask is a function of ``seed`` and is regenerated in
             the backward pass (:func:`attention_dropout_keep`).
-        scale: default hn ** -0.5; must be positive.
+        scale: default hn ** -0.5; in 1e-30 .. 1e30 (the kernels hold it in fp32).
         seed: default: drawn like the other fused attention dropouts (tensor-parallel ranks differ; replayable
             through ``utils.graph_rng``).
 
@@ -119,8 +119,8 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
     if not 0.0 <= dropout_p < 1.0:
         raise ValueError(f"fused_grouped_attention: dropout_p must be in [0, 1), got {dropout_p}")
     scale = float(scale) if scale is not None else query.size(-1) ** -0.5
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"fused_grouped_attention: scale must be positive, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"fused_grouped_attention: scale must be in [1e-30, 1e30], got {scale}")
     if key_lengths is not None:
         if key_lengths.dim() != 1 or key_lengths.size(0) != query.size(1) or key_lengths.is_floating_point():
             raise ValueError("fused_grouped_attention: key_lengths must be an integer [batch] tensor")

@@ -170,6 +170,13 @@ def test_refusals(bad, kw):
         fused_grouped_attention(*bad(q, k, v), **kw)
 
 
+@pytest.mark.parametrize("scale", [1e-60, 1e300, -1.0])
+def test_scales_that_fp32_cannot_hold_are_refused(scale):
+    q, k, v, _ = make(4, 4, 2, 4, 2, 16, torch.float32, "cpu")
+    with pytest.raises(ValueError):
+        fused_grouped_attention(q, k, v, causal=True, scale=scale)
+
+
 def test_keep_flags_match_their_rate_and_differ_by_head_and_seed():
     a = attention_dropout_keep(5, 4, 64, 64, 0.25)
     assert abs(a.float().mean() - 0.75) < 0.02 and not torch.equal(a[0], a[1])
@@ -404,3 +411,10 @@ def test_captured_and_replayed():
         for graph, outs, step, ins in runs:
             for a, b in zip(outs, step()):
                 assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 100.0])
+@pytest.mark.parametrize("sq", [1, 150])
+def test_scales(sq, scale):
+    check(sq, 150, 2, 4, 2, 64, torch.bfloat16, causal=True, scale=scale)
