@@ -19,7 +19,8 @@ namespace {
 
 constexpr int64_t kMaxLen = int64_t(1) << 29;     // queries / keys of a sequence
 constexpr int64_t kMaxStride = int64_t(1) << 24;  // elements between two positions (block offsets are 32-bit)
-constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxTiles = int64_t(1) << 22;
+constexpr int64_t kMaxTokens = int64_t(1) << 26;  // 64 threads each
 
 const int64_t* step_seed(const c10::optional<at::Tensor>& t, const at::Tensor& like, const char* what) {
   if (!t.has_value() || !t->defined()) return nullptr;
@@ -66,8 +67,10 @@ bh::GaArgs ga_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   TORCH_CHECK_VALUE(p >= 0 && p < 1, "grouped attention: dropout must be in [0, 1), got ", p);
   a.sq = (int)q.size(0); a.b = (int)q.size(1); a.np = (int)q.size(2); a.hn = (int)q.size(3);
   a.sk = (int)k.size(0); a.ng = (int)k.size(2);
-  TORCH_CHECK_VALUE(q.size(1) * q.size(2) * ((q.size(0) + 15) / 16 + (k.size(0) + 15) / 16) <= kMaxGrid,
-              "grouped attention: too many rows for one launch");
+  // 128-row tiles of all heads: the largest launch is of 2 * 512 threads a tile, and a launch has fewer than 2^32
+  TORCH_CHECK_VALUE(q.size(1) * q.size(2) * ((q.size(0) + 127) / 128) < kMaxTiles &&
+                        k.size(1) * k.size(2) * ((k.size(0) + 127) / 128) < kMaxTiles,
+                    "grouped attention: too many heads and positions for one launch: query ", q.sizes(), ", key ", k.sizes());
   a.causal = causal;
   TORCH_CHECK_VALUE(window == 0 || (causal && window > 0), "grouped attention: a window needs causal and at least one key");
   a.window = (int)(window > 0 ? std::min(window, 2 * kMaxLen) : 2 * kMaxLen);
@@ -258,9 +261,9 @@ bh::QkRopeArgs rope_args(const at::Tensor& q, const at::Tensor& k, const c10::op
   TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == hn, "qk_norm_rope: query ", q.sizes(),
               " and key ", k.sizes(), " do not fit");
   TORCH_CHECK_VALUE(hn >= 2 && hn <= 512 && hn % 2 == 0, "qk_norm_rope: head_dim must be even and at most 512, got ", hn);
-  TORCH_CHECK_VALUE(q.size(0) * q.size(1) <= 4 * kMaxGrid && q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
-                  q.size(2) <= kMaxLen && k.size(2) <= kMaxLen,
-              "qk_norm_rope: too many tokens or heads");
+  TORCH_CHECK_VALUE(q.size(0) * q.size(1) < kMaxTokens && q.size(0) < kMaxTokens && q.size(1) < kMaxTokens &&
+                        q.size(2) <= kMaxLen && k.size(2) <= kMaxLen,
+                    "qk_norm_rope: fewer than 2^26 tokens only, got ", q.sizes());
   a.s = (int)q.size(0); a.b = (int)q.size(1); a.hn = (int)hn;
   a.heads[0] = (int)q.size(2); a.heads[1] = (int)k.size(2);
   const bool norm = wq.has_value() && wq->defined();

@@ -98,7 +98,8 @@ def fused_grouped_attention(query: torch.Tensor, key: torch.Tensor, value: torch
         query: [sq, b, np, hn]; key, value: [sk, b, ng, hn]. np is a multiple of ng; query head j reads key head
             j // (np / ng). Any strides (views of a fused projection output, transposed batch-first tensors);
             a layout the kernels cannot address is copied (b * heads * hn of 2^24 and more cannot be). On the GPU
-            fp16 / bf16, hn a multiple of 8 up to 128; on the CPU any floating type and head size.
+            fp16 / bf16, hn a multiple of 8 up to 128, b * heads * ceil(s / 128) below 2^22; on the CPU any floating
+            type and head size.
         causal: query i sees keys up to i + sk - sq: the last query is aligned with the last key.
         window: with ``causal``, a query sees at most this many keys, its own position's included.
         key_lengths: int [b]; keys from key_lengths[n] on are not seen and not read (they may hold anything, and

@@ -97,7 +97,8 @@ def fused_qk_norm_rope(query: torch.Tensor, key: torch.Tensor, query_weight: Opt
     the weights.
 
     Args:
-        query, key: fp32 / fp16 / bf16, any strides (head_dim not contiguous: copied), hn even and at most 512.
+        query, key: fp32 / fp16 / bf16, any strides (head_dim not contiguous: copied), hn even and at most
+            512; on the GPU fewer than 2^26 tokens.
         query_weight, key_weight: both or none (no norm); fp32 / fp16 / bf16.
         cos, sin: fp32 [positions, rot / 2] tables (:func:`rotary_tables`), both or none (no rotation). Not
             differentiated.

@@ -418,3 +418,22 @@ def test_captured_and_replayed():
 @pytest.mark.parametrize("sq", [1, 150])
 def test_scales(sq, scale):
     check(sq, 150, 2, 4, 2, 64, torch.bfloat16, causal=True, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("sq, sk, heads", [(1, 1, 1 << 22), (1, 1 << 29, 1), (1 << 29, 1, 1)])
+def test_more_rows_than_a_launch_has_are_refused(sq, sk, heads):
+    q, k = (torch.empty(s, 1, heads, 8, device="cuda", dtype=torch.float16) for s in (sq, sk))
+    with pytest.raises(ValueError):
+        fused_grouped_attention(q, k, k)
+
+
+@gpu
+def test_many_heads_of_single_tokens():
+    """2^29 threads: 2^20 key heads with two query heads each."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(1, 1 << 17, 16, 8, generator=g, device="cuda").bfloat16()
+    k = torch.randn(1, 1 << 17, 8, 8, generator=g, device="cuda").bfloat16()
+    lens = torch.randint(0, 2, (1 << 17,), generator=g, device="cuda", dtype=torch.int32)
+    want = k.repeat_interleave(2, 2) * lens.view(1, -1, 1, 1)  # one key or none
+    assert torch.equal(fused_grouped_attention(q, k, k, key_lengths=lens), want)

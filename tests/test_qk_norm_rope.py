@@ -316,3 +316,10 @@ def test_offset_near_the_end_of_64_bits_is_refused():
         with pytest.raises(ValueError):
             fused_qk_norm_rope(q, q, None, None, cos, sin, offset=offset)
     fused_qk_norm_rope(q, q, None, None, cos, sin, offset=2)
+
+
+@gpu
+def test_more_tokens_than_a_launch_has_are_refused():
+    q = torch.zeros(1, 1, 1, 8, device="cuda").expand(1 << 13, 1 << 13, 1, 8)
+    with pytest.raises(ValueError):
+        fused_qk_norm_rope(q, q, torch.ones(8, device="cuda"), torch.ones(8, device="cuda"))
