@@ -347,10 +347,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
 // heads over 8, half the keys there, take 15 + 4 us (34 MB of K / V); four waves that compute one block while the
 // next is in flight took 25 + 6 us. The waves join through LDS, the splits through an fp32 workspace. The kernel is
 // bound by the latency of its few dependent steps: 256 workgroups of at most 5 blocks a wave. 512 workgroups
-// took 31 us where 256 took 27, 128 took 29 (all keys there).
+// took 31 us where 256 took 27, 128 took 29 (all keys there). Only the blocks that a tile's rows see are walked (8
+// tokens, window 512 of 32768 keys: 10 us, 198 over all keys; 4096 causal tokens, 4 heads: 45 us, 57).
 constexpr int kSplitWaves = 8, kSplitKeys = 32 * kSplitWaves;
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk,
+__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk, int kbeg,
                                                                   float* __restrict__ ws) {
   constexpr int RB = 2 * D, IMG = 32 * RB, KS = D / 16, DN = D / 32, NP = IMG / 1024, NW = kSplitWaves;
   constexpr int OS = D + 4;  // floats of a joined row: 4 of padding keep the 32 rows off one bank
@@ -367,7 +368,15 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int 
   const int nk = seq_keys(a, b), off = a.sk - a.sq;
   const T* K = at<const T>(a.k, b, g);
   const T* V = at<const T>(a.v, b, g);
-  const int k1 = min(nk, split * chunk + chunk), first = split * chunk + wave * 32;
+  // the wave's blocks of the split that some row of the tile sees
+  int k1 = min(nk, kbeg + split * chunk + chunk), first = kbeg + split * chunk + wave * 32;
+  if (a.causal) {
+    const int r0 = rt * 32, r1 = min(r0 + 31, rows - 1), j0 = r0 / a.sq, j1 = r1 / a.sq;
+    const int i0 = j0 == j1 ? r0 - j0 * a.sq : 0, i1 = j0 == j1 ? r1 - j1 * a.sq : a.sq - 1;
+    const int unseen = i0 + off - a.window + 1 - (first + 31);
+    if (unseen > 0) first += (unseen + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
+    k1 = min(k1, i1 + off + 1);
+  }
   const char* kimg = smem + wave * 2 * IMG;
   const char* vimg = kimg + IMG;
   const Stage<D, 32, 1> sk(a.k.st, a.hn, 0, lane), sv(a.v.st, a.hn, 0, lane);
@@ -892,18 +901,20 @@ bool drops(const GaArgs& a) { return a.p_drop > 0. && keep_thresh(a) < 65536u; }
 float keep_scale(const GaArgs& a) { return (float)(1.0 / (1.0 - a.p_drop)); }
 
 struct SplitPlan {
-  int rtiles = 0, splits = 0, chunk = 0;  // splits == 0: the tiled forward
+  int rtiles = 0, splits = 0, chunk = 0, kbeg = 0;  // splits == 0: the tiled forward; keys before kbeg: no one's
 };
 SplitPlan split_plan(const GaArgs& a) {
   SplitPlan p;
   const int64_t tiled = (int64_t)((a.sq + kTileQ - 1) / kTileQ) * a.b * a.np;
   const int64_t rows = (int64_t)(a.np / a.ng) * a.sq, rt = (rows + 31) / 32, probs = rt * a.b * a.ng;
   if (drops(a) || (tiled >= 256 && rows > 64)) return p;
-  const int64_t want = std::max<int64_t>(1, 256 / probs), most = std::max(1, (a.sk + kSplitKeys - 1) / kSplitKeys);
+  if (a.causal) p.kbeg = std::max(0, a.sk - a.sq - a.window + 1) & ~31;
+  const int64_t keys = a.sk - p.kbeg;
+  const int64_t want = std::max<int64_t>(1, 256 / probs), most = (keys + kSplitKeys - 1) / kSplitKeys;
   const int64_t s = std::min(want, most);
   p.rtiles = (int)rt;
-  p.chunk = (int)((((int64_t)a.sk + s - 1) / s + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
-  p.splits = (int)(((int64_t)a.sk + p.chunk - 1) / p.chunk);
+  p.chunk = (int)(((keys + s - 1) / s + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
+  p.splits = (int)((keys + p.chunk - 1) / p.chunk);
   return p;
 }
 
@@ -938,7 +949,7 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
       if constexpr (!DROP) {
         const int64_t probs = (int64_t)a.b * a.ng * p.rtiles;
         hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(64 * kSplitWaves), 0, st, a,
-                           p.rtiles, p.splits, p.chunk, ws);
+                           p.rtiles, p.splits, p.chunk, p.kbeg, ws);
         if (p.splits > 1) {
           constexpr int rpb = kThreads / (D / 4);
           hipLaunchKernelGGL((k_ga_join<T, D>), dim3((unsigned)((probs * 32 + rpb - 1) / rpb)), dim3(kThreads), 0, st,

@@ -437,3 +437,12 @@ def test_many_heads_of_single_tokens():
     lens = torch.randint(0, 2, (1 << 17,), generator=g, device="cuda", dtype=torch.int32)
     want = k.repeat_interleave(2, 2) * lens.view(1, -1, 1, 1)  # one key or none
     assert torch.equal(fused_grouped_attention(q, k, k, key_lengths=lens), want)
+
+
+@gpu
+@pytest.mark.parametrize("window", [1, 33, 700, None])
+@pytest.mark.parametrize("lens", [False, True])
+@pytest.mark.parametrize("shape", [(1, 3001, 2, 8, 2, 64), (37, 1500, 1, 6, 2, 128), (300, 40, 2, 4, 2, 64), (700, 700, 1, 3, 1, 24)])
+def test_split_keys_start_where_the_window_does(shape, lens, window):
+    lens = [shape[1] * 3 // 4] * (shape[2] - 1) + [shape[1] - 1] if lens else None
+    check(*shape, torch.bfloat16, causal=True, window=window, lens=lens)
