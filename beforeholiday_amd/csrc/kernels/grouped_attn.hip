@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_ga_fwd(GaArgs a, int nx, uint32
 // bound by the latency of its few dependent steps: 256 workgroups of at most 5 blocks a wave. 512 workgroups
 // took 31 us where 256 took 27, 128 took 29 (all keys there). Only the blocks that a tile's rows see are walked (8
 // tokens, window 512 of 32768 keys: 10 us, 198 over all keys; 4096 causal tokens, 4 heads: 45 us, 57).
-constexpr int kSplitWaves = 8, kSplitKeys = 32 * kSplitWaves;
+constexpr int kSplitWaves = 8, kSplitKeys = 32 * kSplitWaves, kJoinSerial = 8;
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int rtiles, int splits, int chunk, int kbeg,
                                                                   float* __restrict__ ws) {
@@ -489,45 +489,74 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ga_split(GaArgs a, int 
   if (d0 == 0) a.lse[((int64_t)b * a.np + head) * a.sq + iq] = lw == 0.f ? INFINITY : mm + __log2f(lw);
 }
 
-// joins the splits: D / 4 threads a row, 4 dims each
-template <typename T, int D>
+// Joins the splits: D / 4 threads a row with 4 dims each, GR times over, each group every GR-th split with 4 splits'
+// loads in flight; the groups meet in LDS. GR = 1 for up to kJoinSerial splits, else a workgroup a row. One token, 32
+// heads over 8, 4099 keys, forward with GR = 1 and GR = 8: 4 splits (8 sequences) 27.1 and 27.9 us, 8 splits 18.0 and
+// 17.9 us, 16 splits 13.5 and 12.4 us; 64 splits (1 sequence, 8 heads over 1, 16384 keys) 21.8 and 11.8 us.
+template <typename T, int D, int GR>
 __global__ __launch_bounds__(kThreads) void k_ga_join(GaArgs a, int rtiles, int splits, const float* __restrict__ ws) {
-  constexpr int TPR = D / 4, RPB = kThreads / TPR;
+  constexpr int TPR = D / 4, RPB = kThreads / (TPR * GR);
+  static_assert(GR == 1 || RPB == 1, "a workgroup whose row is behind the last leaves before the barrier");
+  __shared__ float sm[GR], sl[GR];
+  __shared__ f4v so[GR][TPR];
   const int r = a.np / a.ng, rows = r * a.sq, units = a.b * a.ng;
-  const int64_t id = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const int d = (threadIdx.x % TPR) * 4;
-  const int prob = (int)(id / 32), row = (int)(id % 32);
+  const int64_t id = (int64_t)blockIdx.x * RPB + (GR == 1 ? threadIdx.x / TPR : 0);
+  const int prob = (int)(id / 32), row = (int)(id % 32), grp = GR == 1 ? 0 : threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR, d = t * 4;
   if (prob >= units * rtiles) return;
   const int unit = prob % units, grow = prob / units * 32 + row;
   if (grow >= rows) return;
   const float* wo = ws + ((int64_t)prob * splits * 32 + row) * D + d;
   const float* wm = ws + (int64_t)units * rtiles * splits * 32 * D + ((int64_t)prob * splits * 32 + row) * 2;
-  // 4 splits' loads in flight at a time; the running maximum rescales what is already there
+  // the running maximum rescales what is already there
   float mm = -INFINITY, l = 0.f;
   f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < splits; s0 += 4) {
+  auto scale_of = [](float m, float sum, float to) {  // no key: 0; NaN stays
+    return m == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - to);
+  };
+  for (int s0 = grp; s0 < splits; s0 += 4 * GR) {
     float ms[4], ls[4];
     f4v o[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int64_t s = min(s0 + x, splits - 1);
+      const int64_t s = min(s0 + x * GR, splits - 1);
       ms[x] = wm[s * 64];
-      ls[x] = s0 + x < splits ? wm[s * 64 + 1] : 0.f;
+      ls[x] = s0 + x * GR < splits ? wm[s * 64 + 1] : 0.f;
       o[x] = *reinterpret_cast<const f4v*>(wo + s * 32 * D);
     }
     const float mn = fmaxf(mm, fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])));
-    const float corr = mm == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mm - mn);
+    const float corr = scale_of(mm, l, mn);
     mm = mn;
     l *= corr;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= corr;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      if (s0 + x >= splits) break;
-      const float f = ms[x] == -INFINITY ? (ls[x] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms[x] - mm);
+      if (s0 + x * GR >= splits) break;
+      const float f = scale_of(ms[x], ls[x], mm);
       l += f * ls[x];
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] += f * o[x][i];
+    }
+  }
+  if constexpr (GR > 1) {
+    if (t == 0) {
+      sm[grp] = mm;
+      sl[grp] = l;
+    }
+    so[grp][t] = acc;
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int x = 1; x < GR; ++x) mm = fmaxf(mm, sm[x]);
+    l = 0.f;
+    acc = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < GR; ++x) {
+      const float f = scale_of(sm[x], sl[x], mm);
+      l += f * sl[x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += f * so[x][t][i];
     }
   }
   const int b = unit / a.ng, g = unit % a.ng, jj = grow / a.sq, iq = grow - jj * a.sq, head = g * r + jj;
@@ -950,11 +979,13 @@ void ga_forward(int dt, const GaArgs& a, float* ws, hipStream_t st) {
         const int64_t probs = (int64_t)a.b * a.ng * p.rtiles;
         hipLaunchKernelGGL((k_ga_split<T, D>), dim3((unsigned)(probs * p.splits)), dim3(64 * kSplitWaves), 0, st, a,
                            p.rtiles, p.splits, p.chunk, p.kbeg, ws);
-        if (p.splits > 1) {
-          constexpr int rpb = kThreads / (D / 4);
-          hipLaunchKernelGGL((k_ga_join<T, D>), dim3((unsigned)((probs * 32 + rpb - 1) / rpb)), dim3(kThreads), 0, st,
-                             a, p.rtiles, p.splits, ws);
-        }
+        auto join = [&](auto gr) {
+          constexpr int GR = decltype(gr)::value, RPB = kThreads / (D / 4 * GR);
+          hipLaunchKernelGGL((k_ga_join<T, D, GR>), dim3((unsigned)((probs * 32 + RPB - 1) / RPB)), dim3(kThreads), 0,
+                             st, a, p.rtiles, p.splits, ws);
+        };
+        if (p.splits > kJoinSerial) join(std::integral_constant<int, kThreads / (D / 4)>{});
+        else if (p.splits > 1) join(std::integral_constant<int, 1>{});
       }
     } else {
       const int nx = (a.sq + kTileQ - 1) / kTileQ;

@@ -446,3 +446,10 @@ def test_many_heads_of_single_tokens():
 def test_split_keys_start_where_the_window_does(shape, lens, window):
     lens = [shape[1] * 3 // 4] * (shape[2] - 1) + [shape[1] - 1] if lens else None
     check(*shape, torch.bfloat16, causal=True, window=window, lens=lens)
+
+
+@gpu
+@pytest.mark.parametrize("hn", [64, 128])
+@pytest.mark.parametrize("sq, sk, lens", [(1, 2305, None), (3, 20000, None), (1, 20000, [0, 19000]), (40, 9000, [300, 8999])])
+def test_many_splits(sq, sk, lens, hn):
+    check(sq, sk, 2 if lens else 1, 4, 2, hn, torch.bfloat16, lens=lens)
