@@ -350,7 +350,9 @@ struct Plan {
   int64_t gx;
 };
 // A wave takes all passes of a token when there are tokens enough to fill the card (2048 waves), else the
-// token's passes are spread over more waves.
+// token's passes are spread over more waves. persistent (weight gradients: a workgroup has one partial row): the 1024
+// workgroups that are resident at once; 16384 tokens, 32 + 8 heads of 128 in bf16: backward 115 + 6 us, with 512 164 + 4,
+// with 2048 115 + 11 (the second figure adds the partial rows).
 Plan plan(const QkRopeArgs& a, bool persistent) {
   int lpr = 8;
   while (lpr * 8 < a.hn) lpr *= 2;
