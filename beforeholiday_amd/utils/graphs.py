@@ -26,6 +26,20 @@ from typing import Any, Callable, Optional
 import torch
 
 
+def _settle_collectives():
+    """Wait until the RCCL process groups' watchdogs have dropped the collectives that ran so far (the device is
+    synchronized: up to one of their 100 ms periods). A watchdog asks the event of every collective it still holds
+    whether it has passed, and HIP answers that with an error, which ends the process, while the event's stream is being
+    captured; collectives issued under capture are not handed to it."""
+    import torch.distributed as dist
+
+    if not (dist.is_available() and dist.is_initialized()):
+        return
+    for pg, (backend, _) in list(dist.distributed_c10d._world.pg_map.items()):
+        if str(backend) == "nccl":
+            pg._wait_for_pending_works()
+
+
 class GraphedStep:
     """``step = GraphedStep(fn); out = step()`` -- ``fn()`` runs ``warmup`` times eagerly on a side
     stream (so lazy initialisation, bucket building and plan caches reach steady state), then once
@@ -57,6 +71,7 @@ class GraphedStep:
                 self.fn()
         cur.wait_stream(side)
         torch.cuda.synchronize()
+        _settle_collectives()
         t0 = time.perf_counter()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, pool=self.pool, stream=side):

@@ -202,3 +202,40 @@ def test_training_state_includes_group_device_hyperparameters():
     g = opt.param_groups[0]
     assert g["step"].data_ptr() in ptrs and g["lr"].data_ptr() in ptrs
 
+
+def test_capture_waits_for_the_watchdogs_of_rccl_groups(monkeypatch):
+    """Between the warm-up's synchronize and the capture every RCCL group is asked to drop its finished collectives."""
+    import contextlib
+
+    import torch.distributed as dist
+    from beforeholiday_amd.utils import graphs
+
+    calls = []
+
+    class Group:
+        def __init__(self, name):
+            self.name = name
+
+        def _wait_for_pending_works(self):
+            calls.append(self.name)
+
+    class World:
+        pg_map = {Group("a"): ("nccl", None), Group("b"): ("gloo", None), Group("c"): ("nccl", None)}
+
+    class Stream:
+        def wait_stream(self, other):
+            pass
+
+    @contextlib.contextmanager
+    def capture(*a, **kw):
+        calls.append("capture")
+        yield
+
+    monkeypatch.setattr(dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(dist.distributed_c10d, "_world", World)
+    cuda = graphs.torch.cuda
+    for name, f in (("current_stream", Stream), ("default_stream", Stream), ("CUDAGraph", object), ("graph", capture),
+                    ("stream", lambda s: contextlib.nullcontext()), ("synchronize", lambda: calls.append("sync"))):
+        monkeypatch.setattr(cuda, name, f)
+    graphs.GraphedStep(lambda: calls.append("step"), warmup=2).capture()
+    assert calls == ["step", "step", "sync", "a", "c", "capture", "step", "sync"]
